@@ -12,7 +12,10 @@ LIB_PATH = os.environ.get("CM_LIB_PATH") or os.path.join(HERE, "libcleanmarl_hip
 
 NUM_STATS = 8
 STAT_PG, STAT_ENT, STAT_KL, STAT_CLIP, STAT_VLOSS, STAT_COUNT = range(6)
+STAT_LOSS, STAT_KL_REF, STAT_WEIGHT = 4, 6, 7  # cm_token_policy_fwd_bwd
+PREF_LOSS, PREF_CORRECT, PREF_MARGIN, PREF_CHOSEN, PREF_REJECTED, PREF_COUNT = range(6)  # cm_preference_fwd_bwd
 OPT_ADAM, OPT_ADAMW, OPT_SGD, OPT_RMSPROP = 0, 1, 2, 3
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 
 _p = C.c_void_p
 _i = C.c_int
@@ -31,7 +34,21 @@ class OptStep(C.Structure):
                 ("step", C.c_int32), ("opt_kind", C.c_int32), ("stats_out", _p)]
 
 
+class TokenRows(C.Structure):
+    """cm_token_rows_t of include/cleanmarl_hip.h: the rows of logits that the token losses work on."""
+    _fields_ = [("logits", _p), ("ld", _l), ("avail", _p), ("avail_ld", _l), ("token", _p), ("rows", _l),
+                ("vocab", C.c_int32), ("dtype", C.c_int32), ("token_bytes", C.c_int32), ("reserved", C.c_int32), ("temperature", _d)]
+
+
+class AdamW(C.Structure):
+    """cm_adamw_t of include/cleanmarl_hip.h: states and hyper-parameters of one step over a list of tensors."""
+    _fields_ = [("exp_avg", _p), ("exp_avg_sq", _p), ("scale", _p), ("n_blocks", _l),
+                ("lr", _d), ("beta1", _d), ("beta2", _d), ("eps", _d), ("weight_decay", _d), ("max_norm", _d), ("grad_scale", _d),
+                ("out_norm", _p), ("ws", _p), ("ws_bytes", _sz), ("step_dev", _p), ("step", C.c_int32), ("state_bits", C.c_int32)]
+
+
 _po = C.POINTER(OptStep)
+_pt = C.POINTER(TokenRows)
 
 # name -> (restype, argtypes); mirrors include/cleanmarl_hip.h one to one
 SIGNATURES = {
@@ -123,6 +140,15 @@ SIGNATURES = {
     "cm_clock_probe": (_i, [_p]),
     "cm_philox4x32_host": (_i, [_p, _l, _p]),
     "cm_philox4x32_device": (_i, [_p, _l, _p, _p]),
+    "cm_token_workspace_bytes": (_sz, [_l, _i]),
+    "cm_token_logprob": (_i, [_pt, _p, _p, _p, _p, _sz, _p]),
+    "cm_token_logprob_bwd": (_i, [_pt, _p, _p, _p, _p, _p, _l, _p]),
+    "cm_token_policy_fwd_bwd": (_i, [_pt, _p, _p, _p, _p, _d, _d, _d, _d, _p, _l, _p, _p, _p, _sz, _p]),
+    "cm_preference_workspace_bytes": (_sz, [_l, _i, _i]),
+    "cm_preference_fwd_bwd": (_i, [_pt, _p, _i, _p, _d, _d, _i, _d, _p, _l, _p, _p, _p, _p, _sz, _p]),
+    "cm_adamw_state_blocks": (_l, [_l]),
+    "cm_adamw_workspace_bytes": (_sz, [_i]),
+    "cm_adamw_multi_step": (_i, [_p, _i, C.POINTER(AdamW), _p]),
 }
 
 _lib = None

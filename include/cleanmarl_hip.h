@@ -510,6 +510,86 @@ int cm_coma_actor_fwd_bwd_ld(const float* obs, int64_t obs_ld, const uint8_t* av
 /* soft_update (coma_multienvs.py:266-270): target = polyak * src + (1 - polyak) * target. */
 int cm_polyak_update(float* target, const float* src, int64_t n, double polyak, cm_stream_t stream);
 
+/* ---- policies whose action is a token: losses on rows of logits --------------------------------------------------
+ * The counterparts, for logits that the caller's own model has made (thousands of columns, 16 or 32 bits), of what the fused
+ * actor passes above do behind their MLP (cleanmarl/mappo_multienvs.py:172-183, 536-570).  A row of `vocab` logits is divided by
+ * `temperature`; columns with avail == 0 do not take part, whatever the logits hold there (NaN and infinities included), and
+ * get a zero gradient.  A row is LEFT OUT -- log-probability, entropy and gradient 0, not counted -- if its token is negative (padding),
+ * its weight is 0 or none of its columns is available (every logit -inf counts as that); the logits of a row that is left out for its
+ * token or weight are not read.  A token >= vocab gives NaN.  The gradient has the logits' type, is rounded once, and may be
+ * written over the logits (dlogits == logits with the same row stride); any other overlap is refused.  Per-row vectors are fp32 and contiguous.
+ * All sums are formed in a fixed order: the same inputs give the same bits. */
+enum { CM_DTYPE_F32 = 0, CM_DTYPE_F16 = 1, CM_DTYPE_BF16 = 2 };
+typedef struct cm_token_rows {
+    const void* logits;      /* [rows][vocab], row stride ld (elements); aligned to the element only */
+    int64_t ld;
+    const uint8_t* avail;    /* [rows][vocab] or NULL, row stride avail_ld */
+    int64_t avail_ld;
+    const void* token;       /* [rows] int32 or int64: the action taken */
+    int64_t rows;            /* 0 allowed */
+    int32_t vocab;
+    int32_t dtype;           /* CM_DTYPE_*: of logits and dlogits */
+    int32_t token_bytes;     /* 4 or 8 */
+    int32_t reserved;
+    double temperature;
+} cm_token_rows_t;
+/* workspace of the calls below that take one (16-byte aligned, contents irrelevant before and after; calls that may run at the same time
+ * -- two streams, two captured graphs -- need one each) */
+size_t cm_token_workspace_bytes(int64_t rows, int vocab);
+/* log-probability of the token (Categorical.log_prob, mappo_multienvs.py:172-176) and, if entropy != NULL, the entropy of each row;
+ * keep (float [rows][2], may be NULL) holds what cm_token_logprob_bwd needs of the softmax. */
+int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* entropy, float* keep, void* ws, size_t ws_bytes, cm_stream_t stream);
+/* dlogits = d_logp * dlogp/dlogits + d_entropy * dH/dlogits (d_entropy may be NULL; it needs the forward call's entropy) */
+int cm_token_logprob_bwd(const cm_token_rows_t* t, const float* keep, const float* entropy, const float* d_logp, const float* d_entropy,
+                         void* dlogits, int64_t dlogits_ld, cm_stream_t stream);
+/* Clipped policy loss with a KL term, forward and backward (mappo_multienvs.py:536-570 on tokens):
+ *   rho = exp(logp - logp_old), pg = min(adv rho, adv clip(rho, 1 - clip_low, 1 + clip_high)),
+ *   kl = e^d - d - 1 with d = logp_ref - logp (0 without logp_ref),  loss = sum_r weight_r (-pg - entropy_coef H + kl_coef kl)
+ * weight (NULL: ones) carries mask and normalisation (1 / number of tokens, or per sequence).  dlogits = dloss/dlogits.
+ * stats[CM_NUM_STATS]: the weighted sums of slots CM_STAT_PG .. CM_STAT_CLIP as above, CM_STAT_LOSS, CM_STAT_COUNT = rows that count,
+ * CM_STAT_KL_REF = sum weight kl, CM_STAT_WEIGHT = sum weight.  logp (may be NULL) receives the log-probabilities. */
+enum { CM_STAT_LOSS = 4, CM_STAT_KL_REF = 6, CM_STAT_WEIGHT = 7 };
+int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* logp_old, const float* adv, const float* logp_ref, const float* weight,
+                            double clip_low, double clip_high, double kl_coef, double entropy_coef, void* dlogits, int64_t dlogits_ld,
+                            float* logp, float* stats, void* ws, size_t ws_bytes, cm_stream_t stream);
+/* Preference loss on paired log ratios, forward and backward.  Rows of sequence q are [seq_start[q], seq_start[q + 1]) (int32 [2 pairs + 1],
+ * ascending, within [0, rows]); sequence i is the chosen and pairs + i the rejected answer of pair i.  L_q = sum of the sequence's
+ * log-probabilities (64-bit sums; tokens < 0 -- prompts, padding -- are left out), logp_ref [2 pairs] the reference policy's sums,
+ *   margin = (L_i - ref_i) - (L_{P+i} - ref_{P+i}),  z = beta margin
+ *   CM_PREFERENCE_SIGMOID: -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing;   CM_PREFERENCE_SQUARED: (margin - 1/(2 beta))^2
+ * dlogits = scale * d(sum of losses)/dlogits (scale = 1 / pairs: the mean).  Rows in front of the first and behind the last sequence are
+ * not touched.  margin [pairs], seq_logp [2 pairs] may be NULL.  stats[CM_NUM_STATS]: sums over the pairs, slots CM_PREF_*. */
+enum { CM_PREFERENCE_SIGMOID = 0, CM_PREFERENCE_SQUARED = 1 };
+enum { CM_PREF_LOSS = 0, CM_PREF_CORRECT = 1 /* margin > 0 */, CM_PREF_MARGIN = 2, CM_PREF_CHOSEN = 3, CM_PREF_REJECTED = 4, CM_PREF_COUNT = 5 };
+size_t cm_preference_workspace_bytes(int64_t rows, int vocab, int pairs);
+int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* seq_start, int pairs, const float* logp_ref, double beta,
+                          double label_smoothing, int kind, double scale, void* dlogits, int64_t dlogits_ld, float* margin,
+                          float* seq_logp, float* stats, void* ws, size_t ws_bytes, cm_stream_t stream);
+
+/* ---- AdamW over a list of tensors (mappo_multienvs.py:578-594 for parameters that are not one flat vector) ------
+ * One entry per tensor that has a gradient this step.  States live in two arenas of n_blocks blocks of 256 elements; entry t owns the
+ * blocks [t.block, t.block + cm_adamw_state_blocks(t.n)); entries come in ascending block order and do not share blocks.  Arenas are
+ * zeroed once by the caller, 16-byte aligned, and keep zeros behind a tensor's last element.
+ *   state_bits 32: exp_avg, exp_avg_sq are fp32.   8: e4m3 codes (OCP, torch.float8_e4m3fn) of m and of sqrt(v), times scale[block][0] / [1].
+ * max_norm > 0 clips the gradients of ALL entries by their global L2 norm (64-bit sum; after grad_scale); out_norm[0] receives the norm, [1] the coefficient.
+ * copy (may be NULL) receives the new parameter in copy_dtype.  Tensors are contiguous and aligned to their element.
+ * step_dev (device, may be NULL) replaces step for launches that a graph replays: the caller increments it on the stream. */
+typedef struct cm_adamw_tensor {
+    void* param; const void* grad; void* copy;
+    int64_t n, block;
+    int32_t param_dtype, grad_dtype, copy_dtype, reserved;
+} cm_adamw_tensor_t;
+typedef struct cm_adamw {
+    void *exp_avg, *exp_avg_sq; float* scale; int64_t n_blocks;
+    double lr, beta1, beta2, eps, weight_decay, max_norm, grad_scale;
+    float* out_norm; void* ws; size_t ws_bytes;   /* only with max_norm > 0; the workspace needs no initialisation */
+    const int32_t* step_dev;
+    int32_t step, state_bits;
+} cm_adamw_t;
+int64_t cm_adamw_state_blocks(int64_t n);
+size_t cm_adamw_workspace_bytes(int n_tensors);
+int cm_adamw_multi_step(const cm_adamw_tensor_t* tensors, int n_tensors, const cm_adamw_t* o, cm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
