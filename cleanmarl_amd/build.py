@@ -10,7 +10,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Wno-pass-failed"]
 INCREMENTAL = False  # set by `python -m cleanmarl_amd.build -i` (development loop); __graft_entry__.build() always compiles everything
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]  # no v_pk_{add,mul,fma}_f32 from ordinary float code
-FILE_FLAGS = {"cm_token.hip": NO_PACKED_FP32, "cm_adamw.hip": NO_PACKED_FP32}  # per-file extra flags
+FILE_FLAGS = {f"cm_{n}.hip": NO_PACKED_FP32 for n in ("token", "token_f32", "token_f16", "token_bf16", "adamw")}  # per-file extra flags
 
 
 def sources():

@@ -71,30 +71,45 @@ struct TokBF16 {
     }
 };
 
-// elements [j, j + W) of a row as floats; places behind the vocabulary and unavailable ones are -inf, whatever the memory holds there
+// W bytes of avail, as words
+template <int W> struct TokAvail { unsigned a[W / 4]; };
+template <int W>
+__device__ __forceinline__ TokAvail<W> tok_avail(const uint8_t* av, int j) {
+    TokAvail<W> r;
+    if constexpr (W == 8) { const tok_u2_a1 v = *reinterpret_cast<const tok_u2_a1*>(av + j); r.a[0] = v[0]; r.a[1] = v[1]; }
+    else r.a[0] = *reinterpret_cast<const tok_u1_a1*>(av + j);
+    return r;
+}
+// elements [j, j + W) of a row, as they are in memory; places behind the vocabulary are -inf and unavailable
+template <class T>
+__device__ __forceinline__ tok_u4 tok_raw(const typename T::elem* row, int j, int V) {
+    if (j + T::W <= V) return *reinterpret_cast<const typename T::vec*>(row + j);
+    float f[T::W];
+#pragma unroll
+    for (int i = 0; i < T::W; ++i) { f[i] = -INFINITY; if (j + i < V) f[i] = T::get(row[j + i]); }
+    return T::pack(f);
+}
+template <int W>
+__device__ __forceinline__ TokAvail<W> tok_raw_avail(const uint8_t* av, int j, int V) {
+    if (j + W <= V) return tok_avail<W>(av, j);
+    TokAvail<W> r = {};
+#pragma unroll
+    for (int i = 0; i < W; ++i) if (j + i < V) r.a[i >> 2] |= (unsigned)av[j + i] << (8 * (i & 3));
+    return r;
+}
+// unavailable places become -inf, whatever the memory holds there
+template <int W>
+__device__ __forceinline__ void tok_mask(const TokAvail<W>& a, float (&f)[W]) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) f[i] = (a.a[i >> 2] >> (8 * (i & 3)) & 0xffu) ? f[i] : -INFINITY;
+}
 template <class T, bool AV>
-__device__ __forceinline__ void tok_load(const typename T::elem* __restrict__ row, const uint8_t* __restrict__ av, int j, int V, float (&f)[T::W]) {
-    constexpr int W = T::W;
-    if (j + W <= V) {
-        const tok_u4 raw = *reinterpret_cast<const typename T::vec*>(row + j);
-        T::unpack(raw, f);
-        if constexpr (AV) {
-            unsigned a[2];
-            if constexpr (W == 8) { const tok_u2_a1 r = *reinterpret_cast<const tok_u2_a1*>(av + j); a[0] = r[0]; a[1] = r[1]; }
-            else a[0] = *reinterpret_cast<const tok_u1_a1*>(av + j);
-#pragma unroll
-            for (int i = 0; i < W; ++i) f[i] = (a[i >> 2] >> (8 * (i & 3)) & 0xffu) ? f[i] : -INFINITY;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            f[i] = -INFINITY;
-            if (j + i < V && (!AV || av[j + i])) f[i] = T::get(row[j + i]);
-        }
-    }
+__device__ __forceinline__ void tok_load(const typename T::elem* row, const uint8_t* av, int j, int V, float (&f)[T::W]) {
+    T::unpack(tok_raw<T>(row, j, V), f);
+    if constexpr (AV) tok_mask<T::W>(tok_raw_avail<T::W>(av, j, V), f);
 }
 template <class T>
-__device__ __forceinline__ void tok_store(typename T::elem* __restrict__ row, int j, int V, const float (&f)[T::W]) {
+__device__ __forceinline__ void tok_store(typename T::elem* row, int j, int V, const float (&f)[T::W]) {
     constexpr int W = T::W;
     if (j + W <= V) {
         *reinterpret_cast<typename T::vec*>(row + j) = T::pack(f);
@@ -105,81 +120,102 @@ __device__ __forceinline__ void tok_store(typename T::elem* __restrict__ row, in
 }
 
 // ---------------------------------------------------------------- running softmax sums
-// m = max x, s = sum e^t, u = sum t e^t with t = (x - m) / T.  The difference is taken BEFORE the scaling: rows whose logits all sit at
-// the type's lowest value are then uniform rows (t = 0) and not overflows, and for 16-bit logits the difference is nearly always exact.
-// m starts at -FLT_MAX and not at -inf: a row with nothing available keeps s = 0 (that is how it is recognised) without a NaN from inf - inf;
-// a NaN or +inf in an available place ends in s = NaN, which is what it should do.
+// m = max x, s = sum e^t, u = sum t2 e^t with t = (x - m) / T and t2 = t log2(e), the argument of v_exp_f32.  The difference is taken BEFORE
+// the scaling: rows whose logits all sit at the type's lowest value are then uniform rows (t = 0) and not overflows, and for 16-bit
+// logits the difference is nearly always exact.  m starts at -FLT_MAX and not at -inf: a row with nothing available keeps s = 0 (that is how it is
+// recognised) without a NaN from inf - inf; a NaN or +inf in an available place ends in s = NaN, which is what it should do.
 struct TokSum { float m, s, u; };
 
-#define TOK_LOG2E 1.4426950408889634f
-struct TokScale { float nat, bin; };  // 1 / T for natural logarithms, log2(e) / T for v_exp_f32
+constexpr float TOK_LN2 = 0.6931471805599453f, TOK_FAR = -1e20f;  // products with e^t = 0 stay 0 where t2 is clamped to TOK_FAR
+struct TokScale { float nat, bin; };  // 1 / T and log2(e) / T
 
 __device__ __forceinline__ float tok_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // brings `a` to the larger maximum m
 template <bool EN>
-__device__ __forceinline__ void tok_raise(TokSum& a, float m, const TokScale& c) {
-    const float f = tok_exp2((a.m - m) * c.bin);
-    if constexpr (EN) a.u = f * fmaf(fmaxf((a.m - m) * c.nat, -1e30f), a.s, a.u);  // sum (t - d) e^(t - d); the clamp keeps 0 * inf out
+__device__ __forceinline__ void tok_raise(TokSum& a, float m, float bin) {
+    const float d = (a.m - m) * bin, f = tok_exp2(d);
+    if constexpr (EN) a.u = f * fmaf(fmaxf(d, TOK_FAR), a.s, a.u);  // sum (t + d) e^(t + d)
     a.s *= f;
     a.m = m;
 }
 template <bool EN>
-__device__ __forceinline__ void tok_merge(TokSum& a, TokSum b, const TokScale& c) {
+__device__ __forceinline__ void tok_merge(TokSum& a, TokSum b, float bin) {
     const float m = fmaxf(a.m, b.m);
-    tok_raise<EN>(a, m, c);
-    tok_raise<EN>(b, m, c);
+    tok_raise<EN>(a, m, bin);
+    tok_raise<EN>(b, m, bin);
     a.s += b.s;
     if constexpr (EN) a.u += b.u;
 }
 template <bool EN, int W>
-__device__ __forceinline__ void tok_add(TokSum& a, const float (&f)[W], const TokScale& c) {
+__device__ __forceinline__ void tok_add(TokSum& a, const float (&f)[W], float bin) {
     float m = a.m;
 #pragma unroll
     for (int i = 0; i < W; ++i) m = fmaxf(m, f[i]);
-    tok_raise<EN>(a, m, c);
+    tok_raise<EN>(a, m, bin);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float d = f[i] - m, e = tok_exp2(d * c.bin);
+        const float d = (f[i] - m) * bin, e = tok_exp2(d);
         a.s += e;
-        if constexpr (EN) a.u = fmaf(e, fmaxf(d * c.nat, -1e30f), a.u);
+        if constexpr (EN) a.u = fmaf(e, fmaxf(d, TOK_FAR), a.u);
     }
 }
 template <bool EN, int G>
-__device__ __forceinline__ void tok_group(TokSum& a, const TokScale& c) {  // over the G lanes of a group (a power of two, <= 64)
+__device__ __forceinline__ void tok_group(TokSum& a, float bin) {  // over the G lanes of a group (a power of two, <= 64)
 #pragma unroll
     for (int o = G / 2; o > 0; o >>= 1) {
         TokSum b;
         b.m = __shfl_xor(a.m, o, 64);
         b.s = __shfl_xor(a.s, o, 64);
         b.u = EN ? __shfl_xor(a.u, o, 64) : 0.0f;
-        tok_merge<EN>(a, b, c);
+        tok_merge<EN>(a, b, bin);
     }
 }
 // over a workgroup of NW waves; `sh` holds NW entries and is free again when its next use has passed a barrier
 template <bool EN, int NW>
-__device__ __forceinline__ void tok_block(TokSum& a, const TokScale& c, TokSum* sh) {
-    tok_group<EN, 64>(a, c);
+__device__ __forceinline__ void tok_block(TokSum& a, float bin, TokSum* sh) {
+    tok_group<EN, 64>(a, bin);
     if constexpr (NW > 1) {
         if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
         __syncthreads();
-        a = sh[0];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) tok_merge<EN>(a, sh[w], c);  // every thread in the same order: one result
+        a = sh[threadIdx.x & (NW - 1)];
+        tok_group<EN, NW>(a, bin);  // every group of NW lanes in the same order: one result
     }
 }
 
 // ---------------------------------------------------------------- what a row's backward needs
-// dx_j = a [j = token] - b p_j + h p_j (log p_j + H), all already divided by T; p_j = e^t / s
-struct TokGrad { float m, rs, logs, H, a, b, h; int tok; };
+// dx_j = a [j = token] - b p_j + h p_j (log p_j + H), all already divided by T; p_j = e^t rs, log p_j + H = t + K
+struct TokGrad { float m, rs, K, a, b, h; int tok; };
 
 template <class T, bool HE>
-__device__ __forceinline__ void tok_grad(const float (&f)[T::W], int j, const TokGrad& g, const TokScale& c, float (&d)[T::W]) {
+__device__ __forceinline__ void tok_grad(const float (&f)[T::W], int j, const TokGrad& g, float bin, float (&d)[T::W]) {
+    const float brs = -g.b * g.rs, hrs = g.h * g.rs;
 #pragma unroll
     for (int i = 0; i < T::W; ++i) {
-        const float t = f[i] - g.m, p = tok_exp2(t * c.bin) * g.rs;
-        float v = -g.b * p;
-        if constexpr (HE) v = fmaf(g.h * p, fmaxf(t * c.nat, -1e30f) - g.logs + g.H, v);  // p = 0 where t is clamped
-        d[i] = (j + i == g.tok) ? v + g.a : v;
+        const float t = (f[i] - g.m) * bin, e = tok_exp2(t);
+        if constexpr (HE) d[i] = e * fmaf(hrs, fmaxf(fmaf(t, TOK_LN2, g.K), TOK_FAR), brs);  // e = 0 where t is clamped
+        else d[i] = e * brs;
+    }
+    if ((unsigned)(g.tok - j) < (unsigned)T::W) {
+#pragma unroll
+        for (int i = 0; i < T::W; ++i) if (j + i == g.tok) d[i] += g.a;
     }
 }
+
+// ---------------------------------------------------------------- arguments of every kernel of the family
+enum { TOK_LOGP = 0, TOK_BWD = 1, TOK_POLICY = 2 };
+constexpr int TOK_STATS = CM_NUM_STATS, TOK_MAX_GRID = 2048;
+
+struct TokArgs {
+    const void* logits; int64_t ld; const uint8_t* avail; int64_t avail_ld; const void* token; int token_bytes;
+    int64_t rows; int V; TokScale c;
+    float *logp, *entropy; float2* keep;                                     // forward: keep = (m, s), s = 0 for a row that is left out
+    const float2* keep_in; const float *entropy_in, *d_logp, *d_entropy;     // backward
+    void* dlogits; int64_t dld;
+    const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy
+    const int32_t* range_lo; const int32_t* range_hi;                        // preference: only the rows [*range_lo, *range_hi) are touched
+};
+// launches the kernels of one type; returns the number of partial rows of statistics (TOK_POLICY)
+int tok_launch_f32(const TokArgs& a, int mode, bool en, hipStream_t s);
+int tok_launch_f16(const TokArgs& a, int mode, bool en, hipStream_t s);
+int tok_launch_bf16(const TokArgs& a, int mode, bool en, hipStream_t s);

@@ -1,0 +1,254 @@
+// cm_token_rows.h -- the kernels of cm_token.hip for one type of logits (instantiated by cm_token_{f32,f16,bf16}.hip).
+#pragma once
+#include "cm_token.h"
+
+namespace {
+
+__device__ __forceinline__ int64_t tok_token(const TokArgs& a, int64_t r) {
+    return a.token_bytes == 8 ? reinterpret_cast<const int64_t*>(a.token)[r] : (int64_t) reinterpret_cast<const int32_t*>(a.token)[r];
+}
+// preference: whether row r belongs to a sequence at all
+__device__ __forceinline__ bool tok_in_range(const TokArgs& a, int64_t r) { return !a.range_lo || (r >= *a.range_lo && r < *a.range_hi); }
+
+// the token's logit as the sums see it: -inf where it is not available; NaN behind the vocabulary -- an error that must be seen
+template <class T, bool AV>
+__device__ __forceinline__ float tok_logit(const typename T::elem* row, const uint8_t* av, int64_t tok, int V) {
+    if (tok >= V) return NAN;
+    return !AV || av[tok] ? T::get(row[tok]) : -INFINITY;
+}
+
+// scalars of the clipped policy loss of one row: adds its statistics to st (where `add`), returns g = dloss / dlogp and h = the entropy's factor
+struct TokPolicyRow { float old, adv, ref, w; };
+__device__ __forceinline__ TokPolicyRow tok_policy_load(const TokArgs& a, int64_t r) {
+    return {a.logp_old[r], a.adv[r], a.logp_ref ? a.logp_ref[r] : 0.0f, a.weight ? a.weight[r] : 1.0f};
+}
+__device__ __forceinline__ void tok_policy_row(const TokArgs& a, const TokPolicyRow& q, float logp, float H, bool add, double (&st)[TOK_STATS], float& g, float& h) {
+    const float delta = logp - q.old, rho = expf(delta), w = q.w;
+    const float whole = q.adv * rho, cut = q.adv * fminf(fmaxf(rho, a.lo), a.hi);
+    const bool number = whole == whole;
+    const float pg = number ? fminf(whole, cut) : NAN;
+    g = number ? (whole <= cut ? -whole : 0.0f) : NAN;  // torch.min's gradient: a tie inside the borders is the unclipped branch, one outside has adv = 0
+    float loss = -pg - a.ent_coef * H, kl = 0.0f;
+    if (a.logp_ref) {
+        const float d = q.ref - logp, e = expm1f(d);
+        kl = e - d;
+        g -= a.kl_coef * e;
+        loss += a.kl_coef * kl;
+    }
+    g *= w;
+    h = w * a.ent_coef;
+    if (add) {
+        st[CM_STAT_PG] += (double)(w * pg);
+        st[CM_STAT_ENT] += (double)(w * H);
+        st[CM_STAT_KL] += (double)(w * ((rho - 1.0f) - delta));
+        st[CM_STAT_CLIP] += (rho < a.lo || rho > a.hi) ? (double)w : 0.0;
+        st[CM_STAT_LOSS] += (double)(w * loss);
+        st[CM_STAT_COUNT] += 1.0;
+        st[CM_STAT_KL_REF] += (double)(w * kl);
+        st[CM_STAT_WEIGHT] += (double)w;
+    }
+}
+
+// One workgroup walks whole rows: a first sweep for (m, s, u), a second one that reads the row again (it is still in a cache) and writes
+// the gradient.
+template <class T, int MODE, bool AV, bool EN, int NT>
+__global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
+    typedef typename T::elem elem;
+    constexpr int W = T::W, NW = NT / 64;
+    __shared__ TokSum sh[2][NW];
+    double st[TOK_STATS] = {};
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        if (!tok_in_range(a, r)) continue;
+        const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
+        const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
+        const int64_t tok = tok_token(a, r);
+        TokPolicyRow q = {};
+        if (MODE == TOK_POLICY) q = tok_policy_load(a, r);
+        bool live = tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f);
+        TokGrad g = {};
+        if (MODE == TOK_BWD) {
+            const float2 k = a.keep_in[r];
+            live = live && k.y != 0.0f;
+            g.m = k.x; g.rs = 1.0f / k.y;
+            g.a = g.b = (tok >= a.V ? NAN : a.d_logp[r]) * a.c.nat;
+            if (EN) { g.K = a.entropy_in[r] - logf(k.y); g.h = -a.d_entropy[r] * a.c.nat; }
+        } else {
+            TokSum z = {-FLT_MAX, 0.0f, 0.0f};
+            float x = 0.0f;
+            if (live) {
+                x = tok_logit<T, AV>(row, av, tok, a.V);
+                for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
+                    float f[W];
+                    tok_load<T, AV>(row, av, j, a.V, f);
+                    tok_add<EN>(z, f, a.c.bin);
+                }
+                tok_block<EN, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+                turn ^= 1;
+                live = z.s != 0.0f;
+            }
+            float logp = 0.0f, H = 0.0f;
+            if (live) {
+                const float logs = logf(z.s);
+                g.m = z.m; g.rs = 1.0f / z.s;
+                logp = (x - z.m) * a.c.nat - logs;
+                if (EN) { g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K; }
+            }
+            if (MODE == TOK_POLICY && live) {
+                float gg, hh;
+                tok_policy_row(a, q, logp, H, threadIdx.x == 0, st, gg, hh);
+                g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
+            }
+            if (threadIdx.x == 0) {
+                if (a.logp) a.logp[r] = logp;
+                if (EN && a.entropy) a.entropy[r] = H;
+                if (a.keep) a.keep[r] = make_float2(z.m, live ? z.s : 0.0f);
+            }
+        }
+        if (MODE != TOK_LOGP) {
+            g.tok = (int)(live && tok < a.V && (!AV || av[tok]) ? tok : -1);  // an unavailable place has no gradient
+            elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
+            for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
+                float f[W], d[W] = {};
+                if (live) {
+                    tok_load<T, AV>(row, av, j, a.V, f);
+                    tok_grad<T, EN>(f, j, g, a.c.bin, d);
+                }
+                tok_store<T>(drow, j, a.V, d);
+            }
+        }
+    }
+    if (MODE == TOK_POLICY && threadIdx.x == 0)
+        for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
+}
+
+// Short rows: G lanes of a wave hold one row in registers (NV pieces of 16 bytes to a lane), 64 / G rows to a wave.  The row is read once,
+// its exponentials are made once and scaled into the gradient.
+template <class T, int MODE, bool AV, bool EN, int G, int NV>
+__global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
+    typedef typename T::elem elem;
+    constexpr int W = T::W, PER = 256 / G;
+    const int gl = threadIdx.x & (G - 1);  // lane in the group
+    double st[TOK_STATS] = {};
+    for (int64_t r = (int64_t)blockIdx.x * PER + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * PER) {
+        if (!tok_in_range(a, r)) continue;
+        const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
+        const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
+        elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
+        const int64_t tok = tok_token(a, r);
+        TokPolicyRow q = {};
+        if (MODE == TOK_POLICY) q = tok_policy_load(a, r);
+        bool live = tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f);
+        float f[NV][W];
+        float x = 0.0f;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int j = (k * G + gl) * W;
+                if (j < a.V) tok_load<T, AV>(row, av, j, a.V, f[k]);
+                else {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) f[k][i] = -INFINITY;
+                }
+            }
+            if (MODE != TOK_BWD) x = tok_logit<T, AV>(row, av, tok, a.V);
+        }
+        TokGrad g = {};
+        if (MODE == TOK_BWD) {
+            const float2 k = a.keep_in[r];
+            live = live && k.y != 0.0f;
+            g.m = k.x; g.rs = 1.0f / k.y;
+            g.a = g.b = (tok >= a.V ? NAN : a.d_logp[r]) * a.c.nat;
+            if (EN) { g.K = a.entropy_in[r] - logf(k.y); g.h = -a.d_entropy[r] * a.c.nat; }
+        } else {
+            float m = -FLT_MAX, s = 0.0f, u = 0.0f;
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) m = fmaxf(m, f[k][i]);
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int i = 0; i < W; ++i) {
+                        const float t = (f[k][i] - m) * a.c.bin, e = tok_exp2(t);
+                        s += e;
+                        if (EN) u = fmaf(e, fmaxf(t, TOK_FAR), u);
+                    }
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); if (EN) u += __shfl_xor(u, o, 64); }
+                live = s != 0.0f;
+            }
+            float logp = 0.0f, H = 0.0f;
+            if (live) {
+                const float logs = logf(s);
+                g.m = m; g.rs = 1.0f / s;
+                logp = (x - m) * a.c.nat - logs;
+                if (EN) { g.K = -u * g.rs * TOK_LN2; H = logs + g.K; }
+            }
+            if (MODE == TOK_POLICY && live) {
+                float gg, hh;
+                tok_policy_row(a, q, logp, H, gl == 0, st, gg, hh);
+                g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
+            }
+            if (gl == 0) {
+                if (a.logp) a.logp[r] = logp;
+                if (EN && a.entropy) a.entropy[r] = H;
+                if (a.keep) a.keep[r] = make_float2(m, live ? s : 0.0f);
+            }
+        }
+        if (MODE != TOK_LOGP) {
+            g.tok = (int)(live && tok < a.V && (!AV || av[tok]) ? tok : -1);
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int j = (k * G + gl) * W;
+                float d[W] = {};
+                if (live) tok_grad<T, EN>(f[k], j, g, a.c.bin, d);
+                if (j < a.V) tok_store<T>(drow, j, a.V, d);
+            }
+        }
+    }
+    if (MODE == TOK_POLICY) {  // lanes with gl != 0 hold zeros
+        __shared__ double sh[4][TOK_STATS];
+#pragma unroll
+        for (int i = 0; i < TOK_STATS; ++i) {
+            const double v = cm_wave_sum_d(st[i]);
+            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6][i] = v;
+        }
+        __syncthreads();
+        if (threadIdx.x < TOK_STATS) a.part[(int64_t)blockIdx.x * TOK_STATS + threadIdx.x] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+    }
+}
+
+// ---------------------------------------------------------------- choice of a kernel
+inline int tok_grid(int64_t items) { return (int)(items < TOK_MAX_GRID ? (items < 1 ? 1 : items) : TOK_MAX_GRID); }
+
+template <class T, int MODE, bool AV, bool EN>
+int tok_launch4(const TokArgs& a, hipStream_t s) {
+    const int64_t nvec = ((int64_t)a.V + T::W - 1) / T::W;
+#define TOK_SHORT(G, NV) do { const int grid = tok_grid((a.rows + 256 / G - 1) / (256 / G)); \
+        hipLaunchKernelGGL((k_tok_short<T, MODE, AV, EN, G, NV>), dim3(grid), dim3(256), 0, s, a); return grid; } while (0)
+    if (nvec <= 2) TOK_SHORT(1, 2);
+    if (nvec <= 8) TOK_SHORT(4, 2);
+    if (nvec <= 32) TOK_SHORT(16, 2);
+    if (nvec <= 128) TOK_SHORT(64, 2);
+#undef TOK_SHORT
+    const int grid = tok_grid(a.rows);
+    hipLaunchKernelGGL((k_tok_stream<T, MODE, AV, EN, 256>), dim3(grid), dim3(256), 0, s, a);
+    return grid;
+}
+template <class T, int MODE>
+int tok_launch2(const TokArgs& a, bool en, hipStream_t s) {
+    if (a.avail) return en ? tok_launch4<T, MODE, true, true>(a, s) : tok_launch4<T, MODE, true, false>(a, s);
+    return en ? tok_launch4<T, MODE, false, true>(a, s) : tok_launch4<T, MODE, false, false>(a, s);
+}
+template <class T>
+int tok_launch_type(const TokArgs& a, int mode, bool en, hipStream_t s) {
+    if (mode == TOK_LOGP) return tok_launch2<T, TOK_LOGP>(a, en, s);
+    if (mode == TOK_BWD) return tok_launch2<T, TOK_BWD>(a, en, s);
+    return tok_launch2<T, TOK_POLICY>(a, en, s);
+}
+
+}  // namespace
