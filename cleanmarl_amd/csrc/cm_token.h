@@ -34,6 +34,7 @@ struct TokF32 {
     }
 };
 struct TokF16 {
+    static constexpr unsigned NEG_INF = 0xfc00u;
     typedef _Float16 elem;
     typedef tok_u4_a2 vec;
     static constexpr int W = 8;
@@ -54,6 +55,7 @@ struct TokF16 {
     }
 };
 struct TokBF16 {
+    static constexpr unsigned NEG_INF = 0xff80u;
     typedef __bf16 elem;
     typedef tok_u4_a2 vec;
     static constexpr int W = 8;
@@ -102,6 +104,21 @@ template <int W>
 __device__ __forceinline__ void tok_mask(const TokAvail<W>& a, float (&f)[W]) {
 #pragma unroll
     for (int i = 0; i < W; ++i) f[i] = (a.a[i >> 2] >> (8 * (i & 3)) & 0xffu) ? f[i] : -INFINITY;
+}
+// the same on a packed piece
+template <class T>
+__device__ __forceinline__ void tok_mask_raw(const TokAvail<T::W>& a, tok_u4& r) {
+    if constexpr (T::W == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (a.a[0] >> (8 * i) & 0xffu) ? r[i] : 0xff800000u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned two = a.a[i >> 1] >> (16 * (i & 1));
+            const unsigned lo = (two & 0xffu) ? (r[i] & 0xffffu) : T::NEG_INF, hi = (two & 0xff00u) ? (r[i] & 0xffff0000u) : (T::NEG_INF << 16);
+            r[i] = lo | hi;
+        }
+    }
 }
 template <class T, bool AV>
 __device__ __forceinline__ void tok_load(const typename T::elem* row, const uint8_t* av, int j, int V, float (&f)[T::W]) {
@@ -187,18 +204,22 @@ __device__ __forceinline__ void tok_block(TokSum& a, float bin, TokSum* sh) {
 // dx_j = a [j = token] - b p_j + h p_j (log p_j + H), all already divided by T; p_j = e^t rs, log p_j + H = t + K
 struct TokGrad { float m, rs, K, a, b, h; int tok; };
 
-template <class T, bool HE>
-__device__ __forceinline__ void tok_grad(const float (&f)[T::W], int j, const TokGrad& g, float bin, float (&d)[T::W]) {
+template <bool HE, int W>
+__device__ __forceinline__ void tok_grad_rest(const float (&f)[W], const TokGrad& g, float bin, float (&d)[W]) {  // without the token's own term
     const float brs = -g.b * g.rs, hrs = g.h * g.rs;
 #pragma unroll
-    for (int i = 0; i < T::W; ++i) {
+    for (int i = 0; i < W; ++i) {
         const float t = (f[i] - g.m) * bin, e = tok_exp2(t);
         if constexpr (HE) d[i] = e * fmaf(hrs, fmaxf(fmaf(t, TOK_LN2, g.K), TOK_FAR), brs);  // e = 0 where t is clamped
         else d[i] = e * brs;
     }
-    if ((unsigned)(g.tok - j) < (unsigned)T::W) {
+}
+template <bool HE, int W>
+__device__ __forceinline__ void tok_grad(const float (&f)[W], int j, const TokGrad& g, float bin, float (&d)[W]) {
+    tok_grad_rest<HE>(f, g, bin, d);
+    if ((unsigned)(g.tok - j) < (unsigned)W) {
 #pragma unroll
-        for (int i = 0; i < T::W; ++i) if (j + i == g.tok) d[i] += g.a;
+        for (int i = 0; i < W; ++i) if (j + i == g.tok) d[i] += g.a;
     }
 }
 

@@ -168,7 +168,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
     a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws;
-    const int parts = tok_launch(a, t->dtype, TOK_POLICY, true, (hipStream_t)stream);
+    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd");
     hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(256), 0, (hipStream_t)stream, a.part, parts, stats);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd/stats");

@@ -7,6 +7,9 @@ namespace {
 __device__ __forceinline__ int64_t tok_token(const TokArgs& a, int64_t r) {
     return a.token_bytes == 8 ? reinterpret_cast<const int64_t*>(a.token)[r] : (int64_t) reinterpret_cast<const int32_t*>(a.token)[r];
 }
+// an input that no kernel of the launch writes, at an index that is the same for the whole wave: a scalar load.  As a vector load it would be
+// the youngest in the queue, and using it would wait for every piece of a row that was asked for before it.
+template <class X> __device__ __forceinline__ X tok_scalar(const X* p, int64_t i) { return ((const __attribute__((address_space(4))) X*)p)[i]; }
 // preference: whether row r belongs to a sequence at all
 __device__ __forceinline__ bool tok_in_range(const TokArgs& a, int64_t r) { return !a.range_lo || (r >= *a.range_lo && r < *a.range_hi); }
 
@@ -55,6 +58,7 @@ template <class T, int MODE, bool AV, bool EN, int NT>
 __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, NW = NT / 64;
+    constexpr bool ENT = EN || MODE == TOK_POLICY;  // the entropy is a statistic of the policy loss; EN: it has a gradient as well
     __shared__ TokSum sh[2][NW];
     double st[TOK_STATS] = {};
     int turn = 0;
@@ -81,9 +85,9 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
                 for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
                     float f[W];
                     tok_load<T, AV>(row, av, j, a.V, f);
-                    tok_add<EN>(z, f, a.c.bin);
+                    tok_add<ENT>(z, f, a.c.bin);
                 }
-                tok_block<EN, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+                tok_block<ENT, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
                 turn ^= 1;
                 live = z.s != 0.0f;
             }
@@ -92,7 +96,7 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
                 const float logs = logf(z.s);
                 g.m = z.m; g.rs = 1.0f / z.s;
                 logp = (x - z.m) * a.c.nat - logs;
-                if (EN) { g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K; }
+                if (ENT) { g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K; }
             }
             if (MODE == TOK_POLICY && live) {
                 float gg, hh;
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
                 float f[W], d[W] = {};
                 if (live) {
                     tok_load<T, AV>(row, av, j, a.V, f);
-                    tok_grad<T, EN>(f, j, g, a.c.bin, d);
+                    tok_grad<EN>(f, j, g, a.c.bin, d);
                 }
                 tok_store<T>(drow, j, a.V, d);
             }
@@ -128,6 +132,7 @@ template <class T, int MODE, bool AV, bool EN, int G, int NV>
 __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, PER = 256 / G;
+    constexpr bool ENT = EN || MODE == TOK_POLICY;
     const int gl = threadIdx.x & (G - 1);  // lane in the group
     double st[TOK_STATS] = {};
     for (int64_t r = (int64_t)blockIdx.x * PER + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * PER) {
@@ -175,10 +180,10 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
                     for (int i = 0; i < W; ++i) {
                         const float t = (f[k][i] - m) * a.c.bin, e = tok_exp2(t);
                         s += e;
-                        if (EN) u = fmaf(e, fmaxf(t, TOK_FAR), u);
+                        if (ENT) u = fmaf(e, fmaxf(t, TOK_FAR), u);
                     }
 #pragma unroll
-                for (int o = G / 2; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); if (EN) u += __shfl_xor(u, o, 64); }
+                for (int o = G / 2; o > 0; o >>= 1) { s += __shfl_xor(s, o, 64); if (ENT) u += __shfl_xor(u, o, 64); }
                 live = s != 0.0f;
             }
             float logp = 0.0f, H = 0.0f;
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
                 const float logs = logf(s);
                 g.m = m; g.rs = 1.0f / s;
                 logp = (x - m) * a.c.nat - logs;
-                if (EN) { g.K = -u * g.rs * TOK_LN2; H = logs + g.K; }
+                if (ENT) { g.K = -u * g.rs * TOK_LN2; H = logs + g.K; }
             }
             if (MODE == TOK_POLICY && live) {
                 float gg, hh;
@@ -205,7 +210,7 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
             for (int k = 0; k < NV; ++k) {
                 const int j = (k * G + gl) * W;
                 float d[W] = {};
-                if (live) tok_grad<T, EN>(f[k], j, g, a.c.bin, d);
+                if (live) tok_grad<EN>(f[k], j, g, a.c.bin, d);
                 if (j < a.V) tok_store<T>(drow, j, a.V, d);
             }
         }
@@ -222,6 +227,163 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
     }
 }
 
+// Long rows: a workgroup holds a row in registers, NV pieces of 16 bytes to a thread, so that the logits leave memory once.  Workgroups are
+// persistent; a piece's register is refilled with the NEXT row as soon as it is used up (forward only: behind its part of the
+// sums, with a gradient: behind its store), so loads are in flight during all of the arithmetic and no second workgroup is needed to hide them.
+// That only works in straight-line code -- behind a branch the compiler waits for every load there is -- so no load depends on a condition:
+// threads without a piece read the row's last one, and where the next row is left out the current one is read again (from a cache).
+// The first FULL pieces of every thread exist (the choice of the kernel sees to that); the V % W elements behind the last piece are one
+// element of the first threads.
+template <class T, int MODE, bool AV, bool EN, int NT, int NV, int FULL>
+__global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
+    typedef typename T::elem elem;
+    constexpr int W = T::W, NW = NT / 64;
+    constexpr bool ENT = EN || MODE == TOK_POLICY;  // the entropy is a statistic of the policy loss; EN: it has a gradient as well
+    __shared__ TokSum sh[2][NW];
+    double st[TOK_STATS] = {};
+    int turn = 0;
+    const int nfull = a.V / W, tid = threadIdx.x;
+    const bool tail = nfull * W + tid < a.V;
+    const int jt = tail ? nfull * W + tid : a.V - 1;
+    struct Row { int64_t tok; TokPolicyRow q; bool live; };
+    auto scalars = [&](int64_t r) {
+        Row s = {-1, {}, false};
+        if (r < a.rows && (!a.range_lo || (r >= tok_scalar(a.range_lo, 0) && r < tok_scalar(a.range_hi, 0)))) {
+            s.tok = a.token_bytes == 8 ? tok_scalar((const int64_t*)a.token, r) : (int64_t)tok_scalar((const int32_t*)a.token, r);
+            if (MODE == TOK_POLICY)
+                s.q = {tok_scalar(a.logp_old, r), tok_scalar(a.adv, r), a.logp_ref ? tok_scalar(a.logp_ref, r) : 0.0f, a.weight ? tok_scalar(a.weight, r) : 1.0f};
+            s.live = s.tok >= 0 && (MODE != TOK_POLICY || s.q.w != 0.0f);
+        }
+        return s;
+    };
+    auto row_at = [&](int64_t r) { return reinterpret_cast<const elem*>(a.logits) + r * a.ld; };
+    auto av_at = [&](int64_t r) { return AV ? a.avail + r * a.avail_ld : nullptr; };
+    // a scalar base per piece and one vector offset for all: left to itself the compiler keeps an address per piece in registers
+    auto at = [&](const elem* row, int k) {
+        unsigned off = (unsigned)k * NT * 16u;
+        asm volatile("" : "+s"(off));
+        return const_cast<typename T::vec*>(reinterpret_cast<const typename T::vec*>(reinterpret_cast<const char*>(row) + off + (unsigned)tid * 16u));
+    };
+    auto piece = [&](const elem* row, int k) -> tok_u4 {
+        if (k < FULL) return *at(row, k);
+        return reinterpret_cast<const typename T::vec*>(row)[min(tid + k * NT, nfull - 1)];
+    };
+    auto piece_av = [&](const uint8_t* av, int k) { return tok_avail<W>(av, (k < FULL ? tid + k * NT : min(tid + k * NT, nfull - 1)) * W); };
+    tok_u4 raw[NV];
+    TokAvail<W> ok[AV ? NV : 1];
+    elem last;
+    uint8_t last_ok = 1;
+    int64_t r = blockIdx.x;
+    Row now = scalars(r);
+    {
+        const elem* row = row_at(r);
+        const uint8_t* av = av_at(r);
+        last = row[jt];
+        if (AV) last_ok = av[jt];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) { raw[k] = piece(row, k); if (AV) ok[k] = piece_av(av, k); }
+    }
+    for (; r < a.rows; r += gridDim.x) {
+        const Row next = scalars(r + gridDim.x);
+        const elem *row = row_at(r), *nrow = next.live ? row_at(r + gridDim.x) : row;
+        const uint8_t *av = av_at(r), *nav = next.live ? av_at(r + gridDim.x) : av;
+        const int64_t tok = now.tok;
+        const int toki = (int)(tok < 0 ? 0 : (tok < a.V ? tok : a.V - 1));
+        float x = T::get(row[toki]);
+        bool tok_ok = true;
+        if (AV) tok_ok = av[toki] != 0;
+        x = tok < a.V ? (tok_ok ? x : -INFINITY) : NAN;
+        TokSum z = {-FLT_MAX, 0.0f, 0.0f};
+        float lastf = -INFINITY;
+        if (now.live) {
+            lastf = tail && last_ok ? T::get(last) : -INFINITY;
+            const float one[1] = {lastf};
+            tok_add<ENT, 1>(z, one, a.c.bin);
+            if (MODE == TOK_LOGP) { last = nrow[jt]; if (AV) last_ok = nav[jt]; }
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                if (AV) tok_mask_raw<T>(ok[k], raw[k]);
+                float f[W];
+                T::unpack(raw[k], f);
+                if (k >= FULL) {
+                    const bool here = tid + k * NT < nfull;
+#pragma unroll
+                    for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
+                }
+                tok_add<ENT>(z, f, a.c.bin);
+                if (MODE == TOK_LOGP) { raw[k] = piece(nrow, k); if (AV) ok[k] = piece_av(nav, k); }
+                __builtin_amdgcn_sched_barrier(0);  // one piece after the other: interleaved, the floats of all of them would be live at once
+            }
+            tok_block<ENT, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+            turn ^= 1;
+        }
+        const bool live = now.live && z.s != 0.0f;
+        TokGrad g = {};  // all zero: a row that is left out gets zeros
+        float logp = 0.0f, H = 0.0f;
+        if (live) {
+            const float logs = logf(z.s);
+            g.m = z.m; g.rs = 1.0f / z.s;
+            logp = (x - z.m) * a.c.nat - logs;
+            if (ENT) { g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K; }
+            if (MODE == TOK_POLICY) {
+                float gg, hh;
+                tok_policy_row(a, now.q, logp, H, tid == 0, st, gg, hh);
+                g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
+            }
+        }
+        if (tid == 0 && (MODE == TOK_POLICY || tok_in_range(a, r))) {
+            if (a.logp) a.logp[r] = logp;
+            if (EN && a.entropy) a.entropy[r] = H;
+            if (a.keep) a.keep[r] = make_float2(z.m, live ? z.s : 0.0f);
+        }
+        if (MODE == TOK_POLICY) {
+            g.tok = live && tok < a.V && tok_ok ? toki : -1;
+            elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
+            if (now.live) {
+                if (tail) {
+                    float d[1];
+                    const float f[1] = {lastf};
+                    tok_grad_rest<EN>(f, g, a.c.bin, d);
+                    drow[jt] = T::put(d[0]);
+                }
+                last = nrow[jt];
+                if (AV) last_ok = nav[jt];
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    asm volatile("" : "+v"(raw[k]));  // unpacked again: the floats of the first sweep would be kept, at two registers for one
+                    float f[W], d[W];
+                    T::unpack(raw[k], f);
+                    tok_grad_rest<EN>(f, g, a.c.bin, d);
+                    if (k < FULL || tid + k * NT < nfull) *at(drow, k) = T::pack(d);
+                    raw[k] = piece(nrow, k);
+                    if (AV) ok[k] = piece_av(nav, k);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // the token's place once more, by the thread that has just written it: a comparison in every piece would be a branch in every piece
+                if (g.tok >= 0 && tid == (g.tok < nfull * W ? (g.tok / W) & (NT - 1) : g.tok - nfull * W)) {
+                    const float f[1] = {x};
+                    float d[1];
+                    tok_grad_rest<EN>(f, g, a.c.bin, d);
+                    drow[g.tok] = T::put(d[0] + g.a);
+                }
+            } else {
+                if (tail) drow[jt] = T::put(0.0f);
+#pragma unroll
+                for (int k = 0; k < NV; ++k) if (k < FULL || tid + k * NT < nfull) *at(drow, k) = tok_u4{0u, 0u, 0u, 0u};
+            }
+        }
+        if (!now.live) {  // nothing has been used up: the next row replaces what is there
+            last = nrow[jt];
+            if (AV) last_ok = nav[jt];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) { raw[k] = piece(nrow, k); if (AV) ok[k] = piece_av(nav, k); }
+        }
+        now = next;
+    }
+    if (MODE == TOK_POLICY && tid == 0)
+        for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
+}
+
 // ---------------------------------------------------------------- choice of a kernel
 inline int tok_grid(int64_t items) { return (int)(items < TOK_MAX_GRID ? (items < 1 ? 1 : items) : TOK_MAX_GRID); }
 
@@ -235,6 +397,21 @@ int tok_launch4(const TokArgs& a, hipStream_t s) {
     if (nvec <= 32) TOK_SHORT(16, 2);
     if (nvec <= 128) TOK_SHORT(64, 2);
 #undef TOK_SHORT
+    if constexpr (MODE != TOK_BWD) {
+        const int64_t nfull = a.V / T::W;
+        // FULL pieces of every thread exist: nfull > NT * FULL (and nfull >= 1)
+#define TOK_REGS(NT, NV, FULL, PER_CU) do { if (nfull <= NT * NV) { const int grid = (int)(a.rows < 256 * PER_CU ? a.rows : 256 * PER_CU); \
+        hipLaunchKernelGGL((k_tok_regs<T, MODE, AV, EN, NT, NV, FULL>), dim3(grid), dim3(NT), 0, s, a); return grid; } } while (0)
+        TOK_REGS(256, 4, 0, 8);
+        TOK_REGS(256, 8, 4, 4);
+        TOK_REGS(256, 12, 8, 4);
+        TOK_REGS(256, 16, 12, 4);
+        TOK_REGS(512, 12, 8, 2);
+        TOK_REGS(512, 16, 12, 2);
+        TOK_REGS(1024, 12, 8, 1);
+        TOK_REGS(1024, 16, 12, 1);
+#undef TOK_REGS
+    }
     const int grid = tok_grid(a.rows);
     hipLaunchKernelGGL((k_tok_stream<T, MODE, AV, EN, 256>), dim3(grid), dim3(256), 0, s, a);
     return grid;
