@@ -15,6 +15,7 @@ typedef unsigned tok_u1_a1 __attribute__((aligned(1)));
 typedef _Float16 tok_h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 tok_b2 __attribute__((ext_vector_type(2)));
 typedef float tok_f2 __attribute__((ext_vector_type(2)));
+typedef unsigned short tok_s2 __attribute__((ext_vector_type(2)));
 
 struct TokF32 {
     typedef float elem;
@@ -112,13 +113,15 @@ __device__ __forceinline__ void tok_mask_raw(const TokAvail<T::W>& a, tok_u4& r)
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] = (a.a[0] >> (8 * i) & 0xffu) ? r[i] : 0xff800000u;
     } else {
+        const tok_s2 inf = {(unsigned short)T::NEG_INF, (unsigned short)T::NEG_INF}, one = {1, 1};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned two = a.a[i >> 1] >> (16 * (i & 1));
-            const unsigned lo = (two & 0xffu) ? (r[i] & 0xffffu) : T::NEG_INF, hi = (two & 0xff00u) ? (r[i] & 0xffff0000u) : (T::NEG_INF << 16);
-            r[i] = lo | hi;
+        for (int i = 0; i < 4; ++i) {  // two bytes -> two halves of all ones or all zeros
+            const unsigned two = __builtin_amdgcn_perm(0u, a.a[i >> 1], i & 1 ? 0x0c030c02u : 0x0c010c00u);
+            const tok_s2 keep = tok_s2{0, 0} - __builtin_elementwise_min(__builtin_bit_cast(tok_s2, two), one), v = __builtin_bit_cast(tok_s2, (unsigned)r[i]);
+            r[i] = __builtin_bit_cast(unsigned, (v & keep) | (inf & ~keep));
         }
     }
+    asm("" : "+v"(r));  // packed from here on: the compiler would keep the halves apart, in two registers
 }
 template <class T, bool AV>
 __device__ __forceinline__ void tok_load(const typename T::elem* row, const uint8_t* av, int j, int V, float (&f)[T::W]) {

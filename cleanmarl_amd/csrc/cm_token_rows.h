@@ -52,78 +52,176 @@ __device__ __forceinline__ void tok_policy_row(const TokArgs& a, const TokPolicy
     }
 }
 
-// One workgroup walks whole rows: a first sweep for (m, s, u), a second one that reads the row again (it is still in a cache) and writes
-// the gradient.
-template <class T, int MODE, bool AV, bool EN, int NT>
+// Rows that no workgroup can hold: a workgroup walks a row twice, once for (m, s, u) and once, reading it again (a part of it from a cache), to
+// write the gradient.
+template <class T, bool AV, bool EN, int NT>
 __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, NW = NT / 64;
-    constexpr bool ENT = EN || MODE == TOK_POLICY;  // the entropy is a statistic of the policy loss; EN: it has a gradient as well
     __shared__ TokSum sh[2][NW];
     double st[TOK_STATS] = {};
     int turn = 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        if (!tok_in_range(a, r)) continue;
         const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
         const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
         const int64_t tok = tok_token(a, r);
-        TokPolicyRow q = {};
-        if (MODE == TOK_POLICY) q = tok_policy_load(a, r);
-        bool live = tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f);
+        const TokPolicyRow q = tok_policy_load(a, r);
+        bool live = tok >= 0 && q.w != 0.0f;
         TokGrad g = {};
-        if (MODE == TOK_BWD) {
-            const float2 k = a.keep_in[r];
-            live = live && k.y != 0.0f;
-            g.m = k.x; g.rs = 1.0f / k.y;
-            g.a = g.b = (tok >= a.V ? NAN : a.d_logp[r]) * a.c.nat;
-            if (EN) { g.K = a.entropy_in[r] - logf(k.y); g.h = -a.d_entropy[r] * a.c.nat; }
-        } else {
+        float logp = 0.0f;
+        if (live) {
             TokSum z = {-FLT_MAX, 0.0f, 0.0f};
-            float x = 0.0f;
-            if (live) {
-                x = tok_logit<T, AV>(row, av, tok, a.V);
-                for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
-                    float f[W];
-                    tok_load<T, AV>(row, av, j, a.V, f);
-                    tok_add<ENT>(z, f, a.c.bin);
-                }
-                tok_block<ENT, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
-                turn ^= 1;
-                live = z.s != 0.0f;
+            const float x = tok_logit<T, AV>(row, av, tok, a.V);
+            for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
+                float f[W];
+                tok_load<T, AV>(row, av, j, a.V, f);
+                tok_add<true>(z, f, a.c.bin);
             }
-            float logp = 0.0f, H = 0.0f;
+            tok_block<true, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+            turn ^= 1;
+            live = z.s != 0.0f;
             if (live) {
                 const float logs = logf(z.s);
                 g.m = z.m; g.rs = 1.0f / z.s;
                 logp = (x - z.m) * a.c.nat - logs;
-                if (ENT) { g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K; }
-            }
-            if (MODE == TOK_POLICY && live) {
+                g.K = -z.u * g.rs * TOK_LN2;
                 float gg, hh;
-                tok_policy_row(a, q, logp, H, threadIdx.x == 0, st, gg, hh);
+                tok_policy_row(a, q, logp, logs + g.K, threadIdx.x == 0, st, gg, hh);
                 g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
             }
-            if (threadIdx.x == 0) {
-                if (a.logp) a.logp[r] = logp;
-                if (EN && a.entropy) a.entropy[r] = H;
-                if (a.keep) a.keep[r] = make_float2(z.m, live ? z.s : 0.0f);
-            }
         }
-        if (MODE != TOK_LOGP) {
-            g.tok = (int)(live && tok < a.V && (!AV || av[tok]) ? tok : -1);  // an unavailable place has no gradient
-            elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
-            for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
-                float f[W], d[W] = {};
-                if (live) {
-                    tok_load<T, AV>(row, av, j, a.V, f);
-                    tok_grad<EN>(f, j, g, a.c.bin, d);
-                }
-                tok_store<T>(drow, j, a.V, d);
+        if (threadIdx.x == 0 && a.logp) a.logp[r] = logp;
+        g.tok = (int)(live && tok < a.V && (!AV || av[tok]) ? tok : -1);  // an unavailable place has no gradient
+        elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
+        for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
+            float f[W], d[W] = {};
+            if (live) {
+                tok_load<T, AV>(row, av, j, a.V, f);
+                tok_grad<EN>(f, j, g, a.c.bin, d);
             }
+            tok_store<T>(drow, j, a.V, d);
         }
     }
-    if (MODE == TOK_POLICY && threadIdx.x == 0)
+    if (threadIdx.x == 0)
         for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
+}
+
+// Forward only, rows too long for a wave: a workgroup per row, several to a CU, two batches of U pieces to a thread in flight.
+template <class T, bool AV, bool EN, int NT, int U>
+__global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
+    typedef typename T::elem elem;
+    constexpr int W = T::W, NW = NT / 64;
+    __shared__ TokSum sh[2][NW];
+    int turn = 0;
+    const int nfull = a.V / W, tid = threadIdx.x, jt = nfull * W + tid;
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        if (!tok_in_range(a, r)) continue;
+        const int64_t tok = tok_token(a, r);
+        const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
+        const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
+        TokSum z = {-FLT_MAX, 0.0f, 0.0f};
+        float x = 0.0f;
+        if (tok >= 0) {
+            x = tok_logit<T, AV>(row, av, tok, a.V);
+            tok_u4 raw[U];
+            TokAvail<W> ok[AV ? U : 1];
+            auto load = [&](int i0) {  // no load depends on a condition: behind the end the row's last piece is read again
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const int i = min(i0 + k * NT + tid, nfull - 1);
+                    raw[k] = reinterpret_cast<const typename T::vec*>(row)[i];
+                    if (AV) ok[k] = tok_avail<W>(av, i * W);
+                }
+            };
+            load(0);
+            for (int i0 = 0; i0 < nfull; i0 += NT * U) {
+                tok_u4 cur[U];
+#pragma unroll
+                for (int k = 0; k < U; ++k) { if (AV) tok_mask_raw<T>(ok[k], raw[k]); cur[k] = raw[k]; }
+                load(i0 + NT * U);
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    if (i0 + k * NT >= nfull) break;
+                    float f[W];
+                    T::unpack(cur[k], f);
+                    if (i0 + k * NT + NT > nfull) {
+                        const bool here = i0 + k * NT + tid < nfull;
+#pragma unroll
+                        for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
+                    }
+                    tok_add<EN>(z, f, a.c.bin);
+                }
+            }
+            if (jt < a.V && (!AV || av[jt])) { const float one[1] = {T::get(row[jt])}; tok_add<EN, 1>(z, one, a.c.bin); }
+            tok_block<EN, NW>(z, a.c.bin, sh[turn]);
+            turn ^= 1;
+        }
+        if (tid == 0) {
+            const bool live = z.s != 0.0f;
+            const float logs = logf(z.s);
+            if (a.logp) a.logp[r] = live ? (x - z.m) * a.c.nat - logs : 0.0f;
+            if (EN && a.entropy) a.entropy[r] = live ? logs - z.u / z.s * TOK_LN2 : 0.0f;
+            if (a.keep) a.keep[r] = make_float2(z.m, z.s);
+        }
+    }
+}
+
+// Backward only, rows too long for a wave: nothing is summed, so a workgroup takes NT * U pieces of one row, whichever.  The rows come in
+// descending order: the last ones that a forward sweep has read are the ones still in a cache.
+template <class T, bool AV, bool EN, int NT, int U>
+__global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int64_t tiles) {
+    typedef typename T::elem elem;
+    constexpr int W = T::W;
+    const int nfull = a.V / W, tid = threadIdx.x;
+    for (int64_t t = tiles - 1 - blockIdx.x; t >= 0; t -= gridDim.x) {
+        const int64_t r = t / parts;
+        const int part = (int)(t - r * parts);
+        if (!tok_in_range(a, r)) continue;
+        const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
+        elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
+        const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
+        const int64_t tok = tok_token(a, r);
+        const float2 keep = a.keep_in[r];
+        const bool live = tok >= 0 && keep.y != 0.0f;
+        const int i0 = part * NT * U, jt = nfull * W + tid;
+        const bool tail = part == 0 && jt < a.V;
+        if (!live) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) if (i0 + k * NT + tid < nfull) reinterpret_cast<typename T::vec*>(drow)[i0 + k * NT + tid] = tok_u4{0u, 0u, 0u, 0u};
+            if (tail) drow[jt] = T::put(0.0f);
+            continue;
+        }
+        TokGrad g = {};
+        g.m = keep.x; g.rs = 1.0f / keep.y;
+        g.a = g.b = (tok >= a.V ? NAN : a.d_logp[r]) * a.c.nat;
+        if (EN) { g.K = a.entropy_in[r] - logf(keep.y); g.h = -a.d_entropy[r] * a.c.nat; }
+        g.tok = (int)(tok < a.V && (!AV || av[tok]) ? tok : -1);
+        tok_u4 raw[U];
+        TokAvail<W> ok[AV ? U : 1];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = min(i0 + k * NT + tid, nfull - 1);
+            raw[k] = reinterpret_cast<const typename T::vec*>(row)[i];
+            if (AV) ok[k] = tok_avail<W>(av, i * W);
+        }
+        float last[1];
+        last[0] = T::get(row[tail ? jt : a.V - 1]);
+        if (AV) last[0] = av[tail ? jt : a.V - 1] ? last[0] : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int i = i0 + k * NT + tid;
+            if (AV) tok_mask_raw<T>(ok[k], raw[k]);
+            float f[W], d[W];
+            T::unpack(raw[k], f);
+            tok_grad<EN>(f, i * W, g, a.c.bin, d);
+            if (i < nfull) reinterpret_cast<typename T::vec*>(drow)[i] = T::pack(d);
+        }
+        if (tail) {
+            float d[1];
+            tok_grad<EN>(last, jt, g, a.c.bin, d);
+            drow[jt] = T::put(d[0]);
+        }
+    }
 }
 
 // Short rows: G lanes of a wave hold one row in registers (NV pieces of 16 bytes to a lane), 64 / G rows to a wave.  The row is read once,
@@ -228,17 +326,15 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
 }
 
 // Long rows: a workgroup holds a row in registers, NV pieces of 16 bytes to a thread, so that the logits leave memory once.  Workgroups are
-// persistent; a piece's register is refilled with the NEXT row as soon as it is used up (forward only: behind its part of the
-// sums, with a gradient: behind its store), so loads are in flight during all of the arithmetic and no second workgroup is needed to hide them.
+// persistent; a piece's register is refilled with the NEXT row as soon as its gradient is stored, so loads are in flight during all of the arithmetic and no second workgroup is needed to hide them.
 // That only works in straight-line code -- behind a branch the compiler waits for every load there is -- so no load depends on a condition:
 // threads without a piece read the row's last one, and where the next row is left out the current one is read again (from a cache).
 // The first FULL pieces of every thread exist (the choice of the kernel sees to that); the V % W elements behind the last piece are one
 // element of the first threads.
-template <class T, int MODE, bool AV, bool EN, int NT, int NV, int FULL>
+template <class T, bool AV, bool EN, int NT, int NV, int FULL>
 __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, NW = NT / 64;
-    constexpr bool ENT = EN || MODE == TOK_POLICY;  // the entropy is a statistic of the policy loss; EN: it has a gradient as well
     __shared__ TokSum sh[2][NW];
     double st[TOK_STATS] = {};
     int turn = 0;
@@ -248,11 +344,10 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     struct Row { int64_t tok; TokPolicyRow q; bool live; };
     auto scalars = [&](int64_t r) {
         Row s = {-1, {}, false};
-        if (r < a.rows && (!a.range_lo || (r >= tok_scalar(a.range_lo, 0) && r < tok_scalar(a.range_hi, 0)))) {
+        if (r < a.rows) {
             s.tok = a.token_bytes == 8 ? tok_scalar((const int64_t*)a.token, r) : (int64_t)tok_scalar((const int32_t*)a.token, r);
-            if (MODE == TOK_POLICY)
-                s.q = {tok_scalar(a.logp_old, r), tok_scalar(a.adv, r), a.logp_ref ? tok_scalar(a.logp_ref, r) : 0.0f, a.weight ? tok_scalar(a.weight, r) : 1.0f};
-            s.live = s.tok >= 0 && (MODE != TOK_POLICY || s.q.w != 0.0f);
+            s.q = {tok_scalar(a.logp_old, r), tok_scalar(a.adv, r), a.logp_ref ? tok_scalar(a.logp_ref, r) : 0.0f, a.weight ? tok_scalar(a.weight, r) : 1.0f};
+            s.live = s.tok >= 0 && s.q.w != 0.0f;
         }
         return s;
     };
@@ -298,8 +393,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         if (now.live) {
             lastf = tail && last_ok ? T::get(last) : -INFINITY;
             const float one[1] = {lastf};
-            tok_add<ENT, 1>(z, one, a.c.bin);
-            if (MODE == TOK_LOGP) { last = nrow[jt]; if (AV) last_ok = nav[jt]; }
+            tok_add<true, 1>(z, one, a.c.bin);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 if (AV) tok_mask_raw<T>(ok[k], raw[k]);
@@ -310,11 +404,10 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
 #pragma unroll
                     for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
                 }
-                tok_add<ENT>(z, f, a.c.bin);
-                if (MODE == TOK_LOGP) { raw[k] = piece(nrow, k); if (AV) ok[k] = piece_av(nav, k); }
+                tok_add<true>(z, f, a.c.bin);
                 __builtin_amdgcn_sched_barrier(0);  // one piece after the other: interleaved, the floats of all of them would be live at once
             }
-            tok_block<ENT, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+            tok_block<true, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
             turn ^= 1;
         }
         const bool live = now.live && z.s != 0.0f;
@@ -324,19 +417,13 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
             const float logs = logf(z.s);
             g.m = z.m; g.rs = 1.0f / z.s;
             logp = (x - z.m) * a.c.nat - logs;
-            if (ENT) { g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K; }
-            if (MODE == TOK_POLICY) {
-                float gg, hh;
-                tok_policy_row(a, now.q, logp, H, tid == 0, st, gg, hh);
-                g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
-            }
+            g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K;
+            float gg, hh;
+            tok_policy_row(a, now.q, logp, H, tid == 0, st, gg, hh);
+            g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
         }
-        if (tid == 0 && (MODE == TOK_POLICY || tok_in_range(a, r))) {
-            if (a.logp) a.logp[r] = logp;
-            if (EN && a.entropy) a.entropy[r] = H;
-            if (a.keep) a.keep[r] = make_float2(z.m, live ? z.s : 0.0f);
-        }
-        if (MODE == TOK_POLICY) {
+        if (tid == 0 && a.logp) a.logp[r] = logp;
+        {
             g.tok = live && tok < a.V && tok_ok ? toki : -1;
             elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
             if (now.live) {
@@ -380,7 +467,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         }
         now = next;
     }
-    if (MODE == TOK_POLICY && tid == 0)
+    if (tid == 0)
         for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
 }
 
@@ -397,11 +484,23 @@ int tok_launch4(const TokArgs& a, hipStream_t s) {
     if (nvec <= 32) TOK_SHORT(16, 2);
     if (nvec <= 128) TOK_SHORT(64, 2);
 #undef TOK_SHORT
-    if constexpr (MODE != TOK_BWD) {
+    if constexpr (MODE == TOK_BWD) {
+        constexpr int NT = 256, U = 4;
+        const int parts = (int)((a.V / T::W + NT * U - 1) / (NT * U));
+        const int64_t tiles = a.rows * parts;
+        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, a, parts, tiles);
+        return 0;
+    }
+    if constexpr (MODE == TOK_LOGP) {
+        const int grid = (int)(a.rows < (1 << 20) ? a.rows : (1 << 20));
+        hipLaunchKernelGGL((k_tok_sum<T, AV, EN, 256, 2>), dim3(grid), dim3(256), 0, s, a);
+        return grid;
+    }
+    if constexpr (MODE == TOK_POLICY) {
         const int64_t nfull = a.V / T::W;
         // FULL pieces of every thread exist: nfull > NT * FULL (and nfull >= 1)
 #define TOK_REGS(NT, NV, FULL, PER_CU) do { if (nfull <= NT * NV) { const int grid = (int)(a.rows < 256 * PER_CU ? a.rows : 256 * PER_CU); \
-        hipLaunchKernelGGL((k_tok_regs<T, MODE, AV, EN, NT, NV, FULL>), dim3(grid), dim3(NT), 0, s, a); return grid; } } while (0)
+        hipLaunchKernelGGL((k_tok_regs<T, AV, EN, NT, NV, FULL>), dim3(grid), dim3(NT), 0, s, a); return grid; } } while (0)
         TOK_REGS(256, 4, 0, 8);
         TOK_REGS(256, 8, 4, 4);
         TOK_REGS(256, 12, 8, 4);
@@ -412,9 +511,11 @@ int tok_launch4(const TokArgs& a, hipStream_t s) {
         TOK_REGS(1024, 16, 12, 1);
 #undef TOK_REGS
     }
-    const int grid = tok_grid(a.rows);
-    hipLaunchKernelGGL((k_tok_stream<T, MODE, AV, EN, 256>), dim3(grid), dim3(256), 0, s, a);
-    return grid;
+    if constexpr (MODE == TOK_POLICY) {
+        const int grid = tok_grid(a.rows);
+        hipLaunchKernelGGL((k_tok_stream<T, AV, EN, 256>), dim3(grid), dim3(256), 0, s, a);
+        return grid;
+    }
 }
 template <class T, int MODE>
 int tok_launch2(const TokArgs& a, bool en, hipStream_t s) {
