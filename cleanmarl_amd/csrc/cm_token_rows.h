@@ -204,9 +204,8 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
             raw[k] = reinterpret_cast<const typename T::vec*>(row)[i];
             if (AV) ok[k] = tok_avail<W>(av, i * W);
         }
-        float last[1];
-        last[0] = T::get(row[tail ? jt : a.V - 1]);
-        if (AV) last[0] = av[tail ? jt : a.V - 1] ? last[0] : -INFINITY;
+        float last[1] = {-INFINITY};
+        if (tail && (!AV || av[jt])) last[0] = T::get(row[jt]);
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             const int i = i0 + k * NT + tid;
@@ -214,7 +213,7 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
             float f[W], d[W];
             T::unpack(raw[k], f);
             tok_grad<EN>(f, i * W, g, a.c.bin, d);
-            if (i < nfull) reinterpret_cast<typename T::vec*>(drow)[i] = T::pack(d);
+            if (i < nfull) __builtin_nontemporal_store((typename T::vec)T::pack(d), reinterpret_cast<typename T::vec*>(drow) + i);
         }
         if (tail) {
             float d[1];
@@ -331,6 +330,8 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
 // threads without a piece read the row's last one, and where the next row is left out the current one is read again (from a cache).
 // The first FULL pieces of every thread exist (the choice of the kernel sees to that); the V % W elements behind the last piece are one
 // element of the first threads.
+// avail: its bytes for the next row pass through a ring of R pieces in registers into LDS, where each thread finds its own again (kept in
+// registers they would be half as much again as the logits: spills at 1024 threads).
 template <class T, bool AV, bool EN, int NT, int NV, int FULL>
 __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     typedef typename T::elem elem;
@@ -353,31 +354,45 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     };
     auto row_at = [&](int64_t r) { return reinterpret_cast<const elem*>(a.logits) + r * a.ld; };
     auto av_at = [&](int64_t r) { return AV ? a.avail + r * a.avail_ld : nullptr; };
-    // a scalar base per piece and one vector offset for all: left to itself the compiler keeps an address per piece in registers
-    auto at = [&](const elem* row, int k) {
-        unsigned off = (unsigned)k * NT * 16u;
+    // a scalar base per piece and a small vector offset: left to itself the compiler keeps an address per piece in registers
+    auto base = [&](const void* p, unsigned off) {
         asm volatile("" : "+s"(off));
-        return const_cast<typename T::vec*>(reinterpret_cast<const typename T::vec*>(reinterpret_cast<const char*>(row) + off + (unsigned)tid * 16u));
+        return reinterpret_cast<const char*>(p) + off;
     };
+    auto at = [&](const elem* row, int k) { return const_cast<typename T::vec*>(reinterpret_cast<const typename T::vec*>(base(row, k * NT * 16u) + (unsigned)tid * 16u)); };
     auto piece = [&](const elem* row, int k) -> tok_u4 {
         if (k < FULL) return *at(row, k);
-        return reinterpret_cast<const typename T::vec*>(row)[min(tid + k * NT, nfull - 1)];
+        const int slot = min(tid, nfull - 1 - k * NT);  // below zero for a piece that no thread has: the row's last one then
+        return *reinterpret_cast<const typename T::vec*>(base(row, k * NT * 16u) + slot * 16);
     };
-    auto piece_av = [&](const uint8_t* av, int k) { return tok_avail<W>(av, (k < FULL ? tid + k * NT : min(tid + k * NT, nfull - 1)) * W); };
+    auto piece_av = [&](const uint8_t* av, int k) {
+        if (k < FULL) return tok_avail<W>(reinterpret_cast<const uint8_t*>(base(av, k * NT * W) + (unsigned)(tid * W)), 0);
+        const int slot = min(tid, nfull - 1 - k * NT);
+        return tok_avail<W>(reinterpret_cast<const uint8_t*>(base(av, k * NT * W) + slot * W), 0);
+    };
+    constexpr int R = NV < 8 ? NV : 8;
+    __shared__ TokAvail<W> ok[AV ? NV : 1][AV ? NT : 1];
     tok_u4 raw[NV];
-    TokAvail<W> ok[AV ? NV : 1];
+    TokAvail<W> ring[AV ? R : 1];
     elem last;
     uint8_t last_ok = 1;
     int64_t r = blockIdx.x;
     Row now = scalars(r);
-    {
-        const elem* row = row_at(r);
-        const uint8_t* av = av_at(r);
+    auto fill = [&](const elem* row, const uint8_t* av) {  // a whole row at once
         last = row[jt];
         if (AV) last_ok = av[jt];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) { raw[k] = piece(row, k); if (AV) ok[k] = piece_av(av, k); }
-    }
+        for (int k = 0; k < NV; ++k) raw[k] = piece(row, k);
+        if (AV) {
+#pragma unroll
+            for (int k = 0; k < NV + R; ++k) {
+                if (k >= R) ok[k - R][tid] = ring[k % R];
+                if (k < NV) ring[k % R] = piece_av(av, k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    fill(row_at(r), av_at(r));
     for (; r < a.rows; r += gridDim.x) {
         const Row next = scalars(r + gridDim.x);
         const elem *row = row_at(r), *nrow = next.live ? row_at(r + gridDim.x) : row;
@@ -396,7 +411,8 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
             tok_add<true, 1>(z, one, a.c.bin);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                if (AV) tok_mask_raw<T>(ok[k], raw[k]);
+                if (k >= FULL && k * NT >= nfull) break;
+                if (AV) tok_mask_raw<T>(ok[k][tid], raw[k]);
                 float f[W];
                 T::unpack(raw[k], f);
                 if (k >= FULL) {
@@ -405,7 +421,12 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
                     for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
                 }
                 tok_add<true>(z, f, a.c.bin);
-                __builtin_amdgcn_sched_barrier(0);  // one piece after the other: interleaved, the floats of all of them would be live at once
+                asm volatile("" : "+v"(z.m), "+v"(z.s), "+v"(z.u));  // one piece after the other: interleaved, the floats of all of them would be live at once
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (AV) {
+#pragma unroll
+                for (int k = 0; k < R; ++k) ring[k] = piece_av(nav, k);
             }
             tok_block<true, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
             turn ^= 1;
@@ -438,12 +459,17 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     asm volatile("" : "+v"(raw[k]));  // unpacked again: the floats of the first sweep would be kept, at two registers for one
-                    float f[W], d[W];
-                    T::unpack(raw[k], f);
-                    tok_grad_rest<EN>(f, g, a.c.bin, d);
-                    if (k < FULL || tid + k * NT < nfull) *at(drow, k) = T::pack(d);
+                    if (k < FULL || tid + k * NT < nfull) {
+                        float f[W], d[W];
+                        T::unpack(raw[k], f);
+                        tok_grad_rest<EN>(f, g, a.c.bin, d);
+                        __builtin_nontemporal_store((typename T::vec)T::pack(d), at(drow, k));
+                    }
+                    if (AV) {
+                        ok[k][tid] = ring[k % R];
+                        if (k + R < NV) ring[k % R] = piece_av(nav, k + R);
+                    }
                     raw[k] = piece(nrow, k);
-                    if (AV) ok[k] = piece_av(nav, k);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 // the token's place once more, by the thread that has just written it: a comparison in every piece would be a branch in every piece
@@ -459,12 +485,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
                 for (int k = 0; k < NV; ++k) if (k < FULL || tid + k * NT < nfull) *at(drow, k) = tok_u4{0u, 0u, 0u, 0u};
             }
         }
-        if (!now.live) {  // nothing has been used up: the next row replaces what is there
-            last = nrow[jt];
-            if (AV) last_ok = nav[jt];
-#pragma unroll
-            for (int k = 0; k < NV; ++k) { raw[k] = piece(nrow, k); if (AV) ok[k] = piece_av(nav, k); }
-        }
+        if (!now.live) fill(nrow, nav);  // nothing has been used up: the next row replaces what is there
         now = next;
     }
     if (tid == 0)
