@@ -31,7 +31,8 @@ struct AwArgs {
 };
 
 typedef float aw_f4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned aw_u2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned aw_u4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned aw_u2 __attribute__((ext_vector_type(2)));
 typedef _Float16 aw_h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 aw_b2 __attribute__((ext_vector_type(2)));
 typedef float aw_f2 __attribute__((ext_vector_type(2)));
@@ -46,41 +47,44 @@ __device__ __forceinline__ void aw_put(void* p, int64_t i, int dt, float v) {
     else if (dt == CM_DTYPE_F16) reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
     else reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
 }
-// four elements from i on; k of them exist
-__device__ __forceinline__ void aw_load(const void* p, int64_t i, int dt, int k, float (&f)[4]) {
-    if (k >= 4) {
+// eight elements from i on; k of them exist
+__device__ __forceinline__ void aw_load(const void* p, int64_t i, int dt, int k, float (&f)[8]) {
+    if (k >= 8) {
         if (dt == CM_DTYPE_F32) {
-            const aw_f4 r = *reinterpret_cast<const aw_f4*>(reinterpret_cast<const float*>(p) + i);
-            f[0] = r[0]; f[1] = r[1]; f[2] = r[2]; f[3] = r[3];
-        } else {
-            const aw_u2 r = *reinterpret_cast<const aw_u2*>(reinterpret_cast<const uint16_t*>(p) + i);
+            const aw_f4* q = reinterpret_cast<const aw_f4*>(reinterpret_cast<const float*>(p) + i);
+            const aw_f4 r0 = q[0], r1 = q[1];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            for (int j = 0; j < 4; ++j) { f[j] = r0[j]; f[4 + j] = r1[j]; }
+        } else {
+            const aw_u4 r = *reinterpret_cast<const aw_u4*>(reinterpret_cast<const uint16_t*>(p) + i);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
                 if (dt == CM_DTYPE_F16) { const aw_h2 h = __builtin_bit_cast(aw_h2, (unsigned)r[q]); f[2 * q] = (float)h[0]; f[2 * q + 1] = (float)h[1]; }
                 else { f[2 * q] = __uint_as_float(r[q] << 16); f[2 * q + 1] = __uint_as_float(r[q] & 0xffff0000u); }
             }
         }
     } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) f[q] = q < k ? aw_get(p, i + q, dt) : 0.0f;
+        for (int q = 0; q < 8; ++q) f[q] = q < k ? aw_get(p, i + q, dt) : 0.0f;
     }
 }
-__device__ __forceinline__ void aw_store(void* p, int64_t i, int dt, int k, const float (&f)[4]) {
-    if (k >= 4) {
+__device__ __forceinline__ void aw_store(void* p, int64_t i, int dt, int k, const float (&f)[8]) {
+    if (k >= 8) {
         if (dt == CM_DTYPE_F32) {
-            *reinterpret_cast<aw_f4*>(reinterpret_cast<float*>(p) + i) = aw_f4{f[0], f[1], f[2], f[3]};
+            aw_f4* q = reinterpret_cast<aw_f4*>(reinterpret_cast<float*>(p) + i);
+            q[0] = aw_f4{f[0], f[1], f[2], f[3]}; q[1] = aw_f4{f[4], f[5], f[6], f[7]};
         } else {
-            aw_u2 r;
+            aw_u4 r;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            for (int q = 0; q < 4; ++q) {
                 if (dt == CM_DTYPE_F16) r[q] = __builtin_bit_cast(unsigned, aw_h2{(_Float16)f[2 * q], (_Float16)f[2 * q + 1]});
                 else r[q] = __builtin_bit_cast(unsigned, __builtin_convertvector(aw_f2{f[2 * q], f[2 * q + 1]}, aw_b2));
             }
-            *reinterpret_cast<aw_u2*>(reinterpret_cast<uint16_t*>(p) + i) = r;
+            *reinterpret_cast<aw_u4*>(reinterpret_cast<uint16_t*>(p) + i) = r;
         }
     } else {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) if (q < k) aw_put(p, i + q, dt, f[q]);
+        for (int q = 0; q < 8; ++q) if (q < k) aw_put(p, i + q, dt, f[q]);
     }
 }
 
@@ -91,13 +95,16 @@ __device__ __forceinline__ int aw_find(const AwTable& t, int wg) {
     return lo;
 }
 
-__device__ __forceinline__ float aw_wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// maximum over the 32 lanes that hold one block: four rotations within the rows of 16 lanes, then the other row
+template <int ROR> __device__ __forceinline__ float aw_max_ror(float v) {
+    return fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x120 + ROR, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float aw_block_max(float v) {
+    v = aw_max_ror<8>(v); v = aw_max_ror<4>(v); v = aw_max_ror<2>(v); v = aw_max_ror<1>(v);
+    return fmaxf(v, __uint_as_float(__builtin_amdgcn_ds_swizzle(__float_as_uint(v), 0x401f)));
 }
 
-// One wave per block of 256 elements, four to a lane.
+// Half a wave per block of 256 elements, eight to a lane: 16-byte accesses of 16-bit tensors, one 8-byte access of a block's codes.
 template <int BITS>
 __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a) {
 #pragma clang fp contract(off)
@@ -111,31 +118,37 @@ __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a
         inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(a.b2, s)));
     }
     const float coef = a.coef ? a.coef[0] : 1.0f;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int half = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t blocks = (e.n + AW_BLOCK - 1) / AW_BLOCK, b0 = (int64_t)(blockIdx.x - e.first) * AW_CHUNK;
     const int64_t b1 = min(b0 + AW_CHUNK, blocks);
-    for (int64_t b = b0 + wave; b < b1; b += AW_NT / 64) {
-        const int64_t i = b * AW_BLOCK + 4 * lane, at = (e.block + b) * AW_BLOCK + 4 * lane;
+    for (int64_t b = b0 + half; b < b1; b += AW_NT / 32) {
+        const int64_t i = b * AW_BLOCK + 8 * lane, at = (e.block + b) * AW_BLOCK + 8 * lane;
         const int64_t left = e.n - i;
-        const int k = left >= 4 ? 4 : (left > 0 ? (int)left : 0);
-        float p[4], g[4], m[4], r[4];
+        const int k = left >= 8 ? 8 : (left > 0 ? (int)left : 0);
+        float p[8], g[8], m[8], r[8];
+        aw_u2 cm = {}, cr = {};
+        float sm = 0.0f, sr = 0.0f;
+        if (BITS == 8) {
+            cm = reinterpret_cast<const aw_u2*>(a.m)[at / 8]; cr = reinterpret_cast<const aw_u2*>(a.v)[at / 8];
+            sm = a.scale[2 * (e.block + b)]; sr = a.scale[2 * (e.block + b) + 1];
+        }
         aw_load(e.p, i, pd, k, p);
         aw_load(e.g, i, gd, k, g);
-        float sm = 0.0f, sr = 0.0f;
         if (BITS == 32) {
-            aw_load(a.m, at, CM_DTYPE_F32, 4, m);
-            aw_load(a.v, at, CM_DTYPE_F32, 4, r);
+            aw_load(a.m, at, CM_DTYPE_F32, 8, m);
+            aw_load(a.v, at, CM_DTYPE_F32, 8, r);
         } else {
-            sm = a.scale[2 * (e.block + b)]; sr = a.scale[2 * (e.block + b) + 1];
-            const int cm = reinterpret_cast<const int*>(a.m)[at / 4], cr = reinterpret_cast<const int*>(a.v)[at / 4];
-            const aw_f2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8(cm, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(cm, true);
-            const aw_f2 r0 = __builtin_amdgcn_cvt_pk_f32_fp8(cr, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(cr, true);
-            m[0] = m0[0] * sm; m[1] = m0[1] * sm; m[2] = m1[0] * sm; m[3] = m1[1] * sm;
-            r[0] = r0[0] * sr; r[1] = r0[1] * sr; r[2] = r1[0] * sr; r[3] = r1[1] * sr;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const aw_f2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8(cm[q], true);
+                const aw_f2 r0 = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8(cr[q], true);
+                m[4 * q] = m0[0] * sm; m[4 * q + 1] = m0[1] * sm; m[4 * q + 2] = m1[0] * sm; m[4 * q + 3] = m1[1] * sm;
+                r[4 * q] = r0[0] * sr; r[4 * q + 1] = r0[1] * sr; r[4 * q + 2] = r1[0] * sr; r[4 * q + 3] = r1[1] * sr;
+            }
         }
         float tm = 0.0f, tr = 0.0f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 8; ++q) {
             const float gi = (g[q] * a.grad_scale) * coef;
             m[q] = a.beta1 * m[q] + a.omb1 * gi;
             const float v = a.beta2 * (BITS == 32 ? r[q] : r[q] * r[q]) + (a.omb2 * gi) * gi;
@@ -151,19 +164,22 @@ __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a
             aw_store(a.v, at, CM_DTYPE_F32, k, r);
         } else {
             const float f = 1.0f / 448.0f, least = 7.888609052210118e-31f;  // 2^-100: below it a scale would lose bits, and what it scales is nothing
-            tm = aw_wave_max(tm); tr = aw_wave_max(tr);
+            tm = aw_block_max(tm); tr = aw_block_max(tr);
             sm = tm < least ? 0.0f : tm * f; sr = tr < least ? 0.0f : tr * f;
             const float bm = sm > 0.0f ? 1.0f / sm : 0.0f, br = sr > 0.0f ? 1.0f / sr : 0.0f;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < 8; ++q) {
                 m[q] = m[q] * bm;
                 r[q] = r[q] * br;
                 r[q] = (r[q] > 0.0f && r[q] < 0.001953125f) ? 0.001953125f : r[q];
             }
-            int cm = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], 0, false), cr = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
-            cm = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], cm, true); cr = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], cr, true);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                int x = __builtin_amdgcn_cvt_pk_fp8_f32(m[4 * q], m[4 * q + 1], 0, false), y = __builtin_amdgcn_cvt_pk_fp8_f32(r[4 * q], r[4 * q + 1], 0, false);
+                cm[q] = __builtin_amdgcn_cvt_pk_fp8_f32(m[4 * q + 2], m[4 * q + 3], x, true); cr[q] = __builtin_amdgcn_cvt_pk_fp8_f32(r[4 * q + 2], r[4 * q + 3], y, true);
+            }
             // the places behind the tensor hold zeros and stay zero: m = v = g = 0 there
-            reinterpret_cast<int*>(a.m)[at / 4] = cm; reinterpret_cast<int*>(a.v)[at / 4] = cr;
+            reinterpret_cast<aw_u2*>(a.m)[at / 8] = cm; reinterpret_cast<aw_u2*>(a.v)[at / 8] = cr;
             if (lane == 0) { a.scale[2 * (e.block + b)] = sm; a.scale[2 * (e.block + b) + 1] = sr; }
         }
     }
@@ -179,13 +195,13 @@ __global__ __launch_bounds__(AW_NT) void k_adamw_norm(const AwTable t, int chunk
         const AwEntry e = t.e[ti];
         const int gd = (t.kinds[ti] >> 2) & 3;
         const int64_t i0 = (int64_t)(c - e.first) * AW_CHUNK * AW_BLOCK;
-        for (int b = wave; b < AW_CHUNK; b += AW_NT / 64) {
-            const int64_t i = i0 + b * AW_BLOCK + 4 * lane, left = e.n - i;
+        for (int b = threadIdx.x >> 5; b < AW_CHUNK; b += AW_NT / 32) {
+            const int64_t i = i0 + b * AW_BLOCK + 8 * (lane & 31), left = e.n - i;
             if (left <= 0) continue;
-            float g[4];
-            aw_load(e.g, i, gd, left >= 4 ? 4 : (int)left, g);
+            float g[8];
+            aw_load(e.g, i, gd, left >= 8 ? 8 : (int)left, g);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) { const double d = (double)(g[q] * grad_scale); s = fma(d, d, s); }
+            for (int q = 0; q < 8; ++q) { const double d = (double)(g[q] * grad_scale); s = fma(d, d, s); }
         }
     }
     s = cm_wave_sum_d(s);
