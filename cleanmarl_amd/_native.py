@@ -4,6 +4,7 @@ The product path has NO fallback: if the shared library is missing or a call fai
 PyTorch is used only for device memory and streams; every pointer handed to the library is a raw
 ``tensor.data_ptr()``.
 """
+import contextlib
 import ctypes as C
 import os
 
@@ -236,6 +237,21 @@ def stream_ptr(stream=None):
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return C.c_void_p(s.cuda_stream)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on_device(index):
+    """Context in which device `index` is the current one; nothing to enter if it already is (torch.cuda.device costs 1.5 us)."""
+    import torch
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(index):
+    """The current HIP stream of device `index` as an integer (torch.cuda.current_stream() costs 3 us, a tenth of a small call)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 _LOW_PRIORITY = {}

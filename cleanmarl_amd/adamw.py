@@ -17,6 +17,8 @@ _DTYPES = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat1
 _ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("copy", np.uint64), ("n", np.int64), ("block", np.int64),
                    ("param_dtype", np.int32), ("grad_dtype", np.int32), ("copy_dtype", np.int32), ("reserved", np.int32)])  # cm_adamw_tensor_t
 
+_contiguous, _address = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
 
 def _tensor(t, what, like=None):
     if t.dtype not in _DTYPES:
@@ -40,7 +42,7 @@ class MultiAdamW:
         self.params = list(params)
         if not self.params:
             raise ValueError("params: an empty list")
-        self.device = self.params[0].device
+        self.device = self.params[0].device  # the tensor's own: it carries an index
         if self.device.type != "cuda":
             raise ValueError(f"params are on {self.device}: the kernels have no CPU form")
         if state_bits not in (8, 32):
@@ -67,6 +69,13 @@ class MultiAdamW:
         self._m, self._v = torch.zeros(total, **state), torch.zeros(total, **state)
         self.scale = torch.zeros(total // BLOCK, 2, device=self.device) if state_bits == 8 else None
         self.norm = torch.zeros(2, device=self.device)
+        # what does not change from step to step; addresses are read at every step
+        self._shapes, self._dtypes = [p.shape for p in self.params], [p.dtype for p in self.params]
+        self._has_copies = any(c is not None for c in self.copies)
+        self._fixed = np.zeros(len(self.params), _ENTRY)
+        self._fixed["n"], self._fixed["block"] = [p.numel() for p in self.params], self.starts[:-1]
+        self._fixed["param_dtype"] = [_DTYPES[p.dtype] for p in self.params]
+        self._fixed["copy_dtype"] = [0 if c is None else _DTYPES[c.dtype] for c in self.copies]
         self.step_dev = torch.zeros(1, dtype=torch.int32, device=self.device) if capturable else None
 
     # the arenas: tensor i's states are elements [256 * starts[i], 256 * starts[i] + numel)
@@ -89,32 +98,47 @@ class MultiAdamW:
     def step(self, grads=None, grad_scale=1.0):
         """One step on ``grads`` (per parameter a tensor or None; default: each parameter's .grad).  A parameter without a gradient
         is left alone, its states too.  Gradients are read, multiplied by grad_scale on the way, never written."""
-        grads = [p.grad for p in self.params] if grads is None else list(grads)
-        if len(grads) != len(self.params):
-            raise ValueError(f"grads: {len(grads)} for {len(self.params)} params")
+        params, index = self.params, self.device.index
+        grads = [p.grad for p in params] if grads is None else list(grads)
+        if len(grads) != len(params):
+            raise ValueError(f"grads: {len(grads)} for {len(params)} params")
         have = [i for i, g in enumerate(grads) if g is not None]
-        for i in have:
-            _tensor(grads[i], f"grads[{i}]", like=self.params[i])
+        some = len(have) != len(params)
+        if some:
+            params, grads, copies = ([t[i] for i in have] for t in (params, grads, self.copies))
+        else:
+            copies = self.copies
+        fixed = self._fixed[have] if some else self._fixed
+        shapes, kinds = ([t[i] for i in have] for t in (self._shapes, self._dtypes)) if some else (self._shapes, self._dtypes)
+        # the whole list at once (there may be hundreds of tensors); only a list that is not as it should be is looked through
+        if not ([p.shape for p in params] == shapes == [g.shape for g in grads] and [p.dtype for p in params] == kinds and all(map(_contiguous, params))
+                and all(map(_contiguous, grads)) and all(g.get_device() == index and g.dtype in _DTYPES for g in grads)):
+            for i, p, g, shape, kind in zip(have, params, grads, shapes, kinds):
+                if p.shape != shape or p.dtype != kind or not p.is_contiguous():
+                    raise ValueError(f"params[{i}] has another type, shape or layout than at the start")
+                _tensor(g, f"grads[{i}]", like=p)
         table = np.zeros(len(have), _ENTRY)
-        table["param"] = [self.params[i].data_ptr() for i in have]
-        table["grad"] = [grads[i].data_ptr() for i in have]
-        table["copy"] = [0 if self.copies[i] is None else self.copies[i].data_ptr() for i in have]
-        table["n"] = [self.params[i].numel() for i in have]
-        table["block"] = [self.starts[i] for i in have]
-        table["param_dtype"] = [_DTYPES[self.params[i].dtype] for i in have]
-        table["grad_dtype"] = [_DTYPES[grads[i].dtype] for i in have]
-        table["copy_dtype"] = [0 if self.copies[i] is None else _DTYPES[self.copies[i].dtype] for i in have]
+        for name in ("n", "block", "param_dtype", "copy_dtype"):
+            table[name] = fixed[name]
+        table["param"] = list(map(_address, params))
+        table["grad"] = list(map(_address, grads))
+        table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
+        if self._has_copies:
+            if any(c is not None and (c.shape != p.shape or _DTYPES.get(c.dtype) != k or not c.is_contiguous()) for c, p, k in zip(copies, params, fixed["copy_dtype"])):
+                raise ValueError("copies: one has another type, shape or layout than at the start")
+            table["copy"] = [0 if c is None else c.data_ptr() for c in copies]
         lib = N.load()
-        with torch.cuda.device(self.device):
+        with N.on_device(index):
             clip = self.max_norm is not None and self.max_norm > 0
-            ws = torch.empty(max(1, int(lib.cm_adamw_workspace_bytes(len(have)))), dtype=torch.uint8, device=self.device) if clip else None
+            nbytes = lib.cm_adamw_workspace_bytes(len(have)) if clip else 0
+            ws = torch.empty(max(1, nbytes), dtype=torch.uint8, device=self.device) if clip else None
             if self.capturable:
                 self.step_dev.add_(1)
             o = N.AdamW(self._m.data_ptr(), self._v.data_ptr(), None if self.scale is None else self.scale.data_ptr(), self.starts[-1],
                         self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.max_norm if clip else 0.0, grad_scale,
-                        self.norm.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                        self.norm.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
                         None if self.step_dev is None else self.step_dev.data_ptr(), self.steps + 1, self.state_bits)
-            N.check(lib.cm_adamw_multi_step(table.ctypes.data_as(C.c_void_p), len(have), C.byref(o), N.stream_ptr()), "cm_adamw_multi_step")
+            N.check(lib.cm_adamw_multi_step(table.ctypes.data, len(have), C.byref(o), N.raw_stream(index)), "cm_adamw_multi_step")
         self.steps += 1
 
     def load_state(self, exp_avg, second, scale=None, step=0):

@@ -40,6 +40,8 @@ class PreferenceLoss(NamedTuple):
 def _row_stride(t, what):
     """Elements between the rows of a [..., n] tensor whose leading axes collapse into one without a copy."""
     n = t.shape[-1]
+    if t.is_contiguous():
+        return n
     if n > 1 and t.stride(-1) != 1:
         raise ValueError(f"{what}: the last axis must be contiguous, got strides {tuple(t.stride())}")
     axes = [(s, d) for s, d in zip(t.shape[:-1], t.stride()[:-1]) if s != 1]
@@ -51,30 +53,33 @@ def _row_stride(t, what):
     return axes[-1][1]
 
 
-def _vector(t, token, what, dtype=torch.float32):
+def _vector(t, token, what):
+    """Address of an optional fp32 value per row."""
     if t is None:
         return None
-    if t.dtype != dtype or t.shape != token.shape or t.device != token.device or not t.is_contiguous():
-        raise ValueError(f"{what}: need a contiguous {dtype} tensor of shape {tuple(token.shape)} on {token.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t
+    if t.dtype is not torch.float32 or t.shape != token.shape or t.device != token.device or not t.is_contiguous():
+        raise ValueError(f"{what}: need a contiguous float32 tensor of shape {tuple(token.shape)} on {token.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 def _rows(logits, token, avail, temperature):
-    if logits.device.type != "cuda":
-        raise ValueError(f"logits are on {logits.device}: the kernels have no CPU form")
-    if logits.dtype not in _DTYPES:
+    device, shape = logits.device, logits.shape
+    if device.type != "cuda":
+        raise ValueError(f"logits are on {device}: the kernels have no CPU form")
+    dtype = _DTYPES.get(logits.dtype)
+    if dtype is None:
         raise ValueError(f"logits: float32, float16 or bfloat16, got {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[-1] < 1 or token.shape != logits.shape[:-1]:
-        raise ValueError(f"token: need shape {tuple(logits.shape[:-1])} for logits {tuple(logits.shape)}, got {tuple(token.shape)}")
-    if token.dtype not in (torch.int32, torch.int64) or token.device != logits.device or not token.is_contiguous():
-        raise ValueError(f"token: need a contiguous int32 or int64 tensor on {logits.device}, got {token.dtype} on {token.device}")
-    ld, av, av_ld = _row_stride(logits, "logits"), None, 0
+    if not shape or shape[-1] < 1 or token.shape != shape[:-1]:
+        raise ValueError(f"token: need shape {tuple(shape[:-1])} for logits {tuple(shape)}, got {tuple(token.shape)}")
+    width = 8 if token.dtype is torch.int64 else 4 if token.dtype is torch.int32 else 0
+    if not width or token.device != device or not token.is_contiguous():
+        raise ValueError(f"token: need a contiguous int32 or int64 tensor on {device}, got {token.dtype} on {token.device}")
+    av, av_ld = None, 0
     if avail is not None:
-        if avail.dtype not in (torch.uint8, torch.bool) or avail.shape != logits.shape or avail.device != logits.device:
-            raise ValueError(f"avail: need uint8 or bool of shape {tuple(logits.shape)} on {logits.device}, got {avail.dtype} {tuple(avail.shape)} on {avail.device}")
+        if avail.dtype not in (torch.uint8, torch.bool) or avail.shape != shape or avail.device != device:
+            raise ValueError(f"avail: need uint8 or bool of shape {tuple(shape)} on {device}, got {avail.dtype} {tuple(avail.shape)} on {avail.device}")
         av, av_ld = avail.data_ptr(), _row_stride(avail, "avail")
-    return N.TokenRows(logits.data_ptr(), ld, av, av_ld, token.data_ptr(), token.numel(), logits.shape[-1], _DTYPES[logits.dtype],
-                       token.element_size(), 0, float(temperature))
+    return N.TokenRows(logits.data_ptr(), _row_stride(logits, "logits"), av, av_ld, token.data_ptr(), token.numel(), shape[-1], dtype, width, 0, temperature)
 
 
 def _grad(out, logits):
@@ -87,7 +92,7 @@ def _grad(out, logits):
 
 
 def _workspace(nbytes, device):
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
 
 def token_logprob(logits, token, avail=None, temperature=1.0, entropy=False, keep=False):
@@ -95,13 +100,16 @@ def token_logprob(logits, token, avail=None, temperature=1.0, entropy=False, kee
 
     Replaces Categorical(logits).log_prob / .entropy (cleanmarl/mappo_multienvs.py:172-176, 549-550): one pass over the logits."""
     rows = _rows(logits, token, avail, temperature)
-    lib = N.load()
-    with torch.cuda.device(logits.device):
-        new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
-        r = TokenLogProb(new(*token.shape), new(*token.shape) if entropy else None, new(*token.shape, 2) if keep else None)
-        ws = _workspace(lib.cm_token_workspace_bytes(rows.rows, rows.vocab), logits.device)
-        N.check(lib.cm_token_logprob(C.byref(rows), N.ptr(r.logp), N.ptr(r.entropy), N.ptr(r.keep), N.ptr(ws), ws.numel(), N.stream_ptr()), "cm_token_logprob")
-    return r
+    lib, device, index = N.load(), logits.device, logits.get_device()
+    with N.on_device(index):
+        logp = torch.empty(token.shape, dtype=torch.float32, device=device)
+        H = torch.empty(token.shape, dtype=torch.float32, device=device) if entropy else None
+        kept = torch.empty((*token.shape, 2), dtype=torch.float32, device=device) if keep else None
+        nbytes = lib.cm_token_workspace_bytes(rows.rows, rows.vocab)
+        ws = _workspace(nbytes, device)
+        N.check(lib.cm_token_logprob(C.byref(rows), logp.data_ptr(), None if H is None else H.data_ptr(), None if kept is None else kept.data_ptr(),
+                                     ws.data_ptr(), nbytes, N.raw_stream(index)), "cm_token_logprob")
+    return TokenLogProb(logp, H, kept)
 
 
 def token_logprob_bwd(logits, token, forward, d_logp, d_entropy=None, avail=None, temperature=1.0, out=None):
@@ -114,14 +122,12 @@ def token_logprob_bwd(logits, token, forward, d_logp, d_entropy=None, avail=None
         raise ValueError("forward: need the result of token_logprob(..., keep=True) for these rows")
     if d_entropy is not None and forward.entropy is None:
         raise ValueError("d_entropy: the forward call has to compute the entropy (entropy=True)")
-    _vector(d_logp, token, "d_logp")
-    _vector(d_entropy, token, "d_entropy")
+    dl, dh = _vector(d_logp, token, "d_logp"), _vector(d_entropy, token, "d_entropy")
     H = _vector(forward.entropy, token, "forward.entropy") if d_entropy is not None else None
-    lib = N.load()
-    with torch.cuda.device(logits.device):
+    lib, index = N.load(), logits.get_device()
+    with N.on_device(index):
         out, ld = _grad(out, logits)
-        N.check(lib.cm_token_logprob_bwd(C.byref(rows), N.ptr(forward.keep), N.ptr(H), N.ptr(d_logp), N.ptr(d_entropy), N.ptr(out), ld, N.stream_ptr()),
-                "cm_token_logprob_bwd")
+        N.check(lib.cm_token_logprob_bwd(C.byref(rows), forward.keep.data_ptr(), H, dl, dh, out.data_ptr(), ld, N.raw_stream(index)), "cm_token_logprob_bwd")
     return out
 
 
@@ -133,17 +139,17 @@ def policy_loss_fwd_bwd(logits, token, logp_old, adv, logp_ref=None, weight=None
     rho = exp(logp - logp_old), d = logp_ref - logp.  ``weight`` carries mask and normalisation (None: ones).  All per-row tensors have
     token's shape.  ``out``: where the gradient goes; the logits themselves are allowed."""
     rows = _rows(logits, token, avail, temperature)
-    for t, what in ((logp_old, "logp_old"), (adv, "adv"), (logp_ref, "logp_ref"), (weight, "weight")):
-        _vector(t, token, what)
-    lib = N.load()
-    with torch.cuda.device(logits.device):
+    old, ad = _vector(logp_old, token, "logp_old"), _vector(adv, token, "adv")
+    ref, w = _vector(logp_ref, token, "logp_ref"), _vector(weight, token, "weight")
+    lib, device, index = N.load(), logits.device, logits.get_device()
+    with N.on_device(index):
         out, ld = _grad(out, logits)
-        f32 = dict(dtype=torch.float32, device=logits.device)
-        stats, logp = torch.empty(N.NUM_STATS, **f32), torch.empty(token.shape, **f32)
-        ws = _workspace(lib.cm_token_workspace_bytes(rows.rows, rows.vocab), logits.device)
-        N.check(lib.cm_token_policy_fwd_bwd(C.byref(rows), N.ptr(logp_old), N.ptr(adv), N.ptr(logp_ref), N.ptr(weight), clip_low, clip_high, kl_coef,
-                                            entropy_coef, N.ptr(out), ld, N.ptr(logp), N.ptr(stats), N.ptr(ws), ws.numel(), N.stream_ptr()),
-                "cm_token_policy_fwd_bwd")
+        stats = torch.empty(N.NUM_STATS, dtype=torch.float32, device=device)
+        logp = torch.empty(token.shape, dtype=torch.float32, device=device)
+        nbytes = lib.cm_token_workspace_bytes(rows.rows, rows.vocab)
+        ws = _workspace(nbytes, device)
+        N.check(lib.cm_token_policy_fwd_bwd(C.byref(rows), old, ad, ref, w, clip_low, clip_high, kl_coef, entropy_coef, out.data_ptr(), ld, logp.data_ptr(),
+                                            stats.data_ptr(), ws.data_ptr(), nbytes, N.raw_stream(index)), "cm_token_policy_fwd_bwd")
     return PolicyLoss(stats, out, logp)
 
 
@@ -166,15 +172,17 @@ def preference_loss_fwd_bwd(logits, token, seq_start, logp_ref, beta=0.1, label_
     pairs = n // 2
     if logp_ref.dtype != torch.float32 or logp_ref.shape != (2 * pairs,) or logp_ref.device != logits.device or not logp_ref.is_contiguous():
         raise ValueError(f"logp_ref: need float32 [{2 * pairs}] on {logits.device}, got {logp_ref.dtype} {tuple(logp_ref.shape)} on {logp_ref.device}")
-    lib = N.load()
-    with torch.cuda.device(logits.device):
+    lib, device, index = N.load(), logits.device, logits.get_device()
+    with N.on_device(index):
         if out is None:
             out = torch.zeros_like(logits, memory_format=torch.contiguous_format)
         out, ld = _grad(out, logits)
-        f32 = dict(dtype=torch.float32, device=logits.device)
-        stats, margin, seq_logp = torch.empty(N.NUM_STATS, **f32), torch.empty(pairs, **f32), torch.empty(2 * pairs, **f32)
-        ws = _workspace(lib.cm_preference_workspace_bytes(rows.rows, rows.vocab, pairs), logits.device)
-        N.check(lib.cm_preference_fwd_bwd(C.byref(rows), N.ptr(seq_start), pairs, N.ptr(logp_ref), beta, label_smoothing, _KINDS[kind],
-                                          1.0 / pairs if scale is None else scale, N.ptr(out), ld, N.ptr(margin), N.ptr(seq_logp), N.ptr(stats),
-                                          N.ptr(ws), ws.numel(), N.stream_ptr()), "cm_preference_fwd_bwd")
+        stats = torch.empty(N.NUM_STATS, dtype=torch.float32, device=device)
+        margin = torch.empty(pairs, dtype=torch.float32, device=device)
+        seq_logp = torch.empty(2 * pairs, dtype=torch.float32, device=device)
+        nbytes = lib.cm_preference_workspace_bytes(rows.rows, rows.vocab, pairs)
+        ws = _workspace(nbytes, device)
+        N.check(lib.cm_preference_fwd_bwd(C.byref(rows), seq_start.data_ptr(), pairs, logp_ref.data_ptr(), beta, label_smoothing, _KINDS[kind],
+                                          1.0 / pairs if scale is None else scale, out.data_ptr(), ld, margin.data_ptr(), seq_logp.data_ptr(),
+                                          stats.data_ptr(), ws.data_ptr(), nbytes, N.raw_stream(index)), "cm_preference_fwd_bwd")
     return PreferenceLoss(stats, out, margin, seq_logp)
