@@ -203,6 +203,70 @@ __device__ __forceinline__ void tok_block(TokSum& a, float bin, TokSum* sh) {
     }
 }
 
+// ---------------------------------------------------------------- the same, cheaper, for rows of ordinary size
+// e^t = 2^(x c - M) with c = log2(e) / T: one fused multiply-add and one v_exp_f32.  M is any number near the row's maximum times c: floats have
+// exponents to spare, so M follows the maximum only when that has run TOK_SLACK ahead, and the rescaling costs next to nothing.  M's own
+// rounding is a factor common to every e^t of the row and cancels in e^t / s and in x c - M - log2 s.  What this form cannot do -- rows
+// without a finite sum, logits so large that x c - M has no correct places, -inf beside an entropy (0 * -inf) -- shows in (M, s, u) and is done over with TokSum.
+struct TokRun { float M, s, u; };
+constexpr float TOK_START = -1.2676506e30f /* -2^100 */, TOK_SLACK = 16.0f, TOK_LARGE = 1048576.0f /* 2^20: the places behind x c - M are then at least 2^-4 */;
+
+template <bool EN>
+__device__ __forceinline__ void run_raise(TokRun& a, float M) {
+    const float d = a.M - M, f = tok_exp2(d);
+    if constexpr (EN) a.u = f * fmaf(fmaxf(d, TOK_FAR), a.s, a.u);
+    a.s *= f;
+    a.M = M;
+}
+// CLAMP: -inf among the logits is ordinary (unavailable columns), its product with e^t = 0 must not be NaN
+template <bool EN, bool CLAMP, int W>
+__device__ __forceinline__ void run_add(TokRun& a, const float (&f)[W], float c) {
+    float m = f[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) m = fmaxf(m, f[i]);
+    m *= c;
+    if (m > a.M + TOK_SLACK) run_raise<EN>(a, m);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        const float t = fmaf(f[i], c, -a.M), e = tok_exp2(t);
+        a.s += e;
+        if constexpr (EN) a.u = fmaf(e, CLAMP ? fmaxf(t, TOK_FAR) : t, a.u);
+    }
+}
+template <bool EN>
+__device__ __forceinline__ void run_merge(TokRun& a, TokRun b) {
+    const float M = fmaxf(a.M, b.M);
+    run_raise<EN>(a, M);
+    run_raise<EN>(b, M);
+    a.s += b.s;
+    if constexpr (EN) a.u += b.u;
+}
+template <bool EN, int G>
+__device__ __forceinline__ void run_group(TokRun& a) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) {
+        TokRun b;
+        b.M = __shfl_xor(a.M, o, 64);
+        b.s = __shfl_xor(a.s, o, 64);
+        b.u = EN ? __shfl_xor(a.u, o, 64) : 0.0f;
+        run_merge<EN>(a, b);
+    }
+}
+template <bool EN, int NW>
+__device__ __forceinline__ void run_block(TokRun& a, TokRun* sh) {  // sh: as in tok_block
+    run_group<EN, 64>(a);
+    if constexpr (NW > 1) {
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = sh[threadIdx.x & (NW - 1)];
+        run_group<EN, NW>(a);
+    }
+}
+template <bool EN>
+__device__ __forceinline__ bool run_ordinary(const TokRun& a) {
+    return a.s > 0.0f && a.s < INFINITY && fabsf(a.M) <= TOK_LARGE && (!EN || fabsf(a.u) < INFINITY);
+}
+
 // ---------------------------------------------------------------- what a row's backward needs
 // dx_j = a [j = token] - b p_j + h p_j (log p_j + H), all already divided by T; p_j = e^t rs, log p_j + H = t + K
 struct TokGrad { float m, rs, K, a, b, h; int tok; };
@@ -226,6 +290,48 @@ __device__ __forceinline__ void tok_grad(const float (&f)[W], int j, const TokGr
     }
 }
 
+// The same in the form of TokRun: 2^(x c - M) rs.  16-bit gradients take the row's factor into the exponent (its rounding there, at most
+// 2^-16 of the value, is nothing beside theirs) and its sign into the packed pieces, unless M is so large that its places would be lost.
+struct RunGrad { float M, brs, hrs, K, shift; unsigned sign; bool fold; };
+template <class T, bool HE>
+__device__ __forceinline__ RunGrad run_grad_row(float M, float s, float K, float b, float h) {
+    RunGrad g;
+    const float rs = 1.0f / s;
+    g.M = M; g.K = K; g.brs = -b * rs; g.hrs = h * rs;
+    g.shift = log2f(fabsf(b)) - log2f(s) - M;  // b = 0: -inf, and every 2^ is 0
+    g.sign = (__float_as_uint(-b) >> 31) ? 0x80008000u : 0u;
+    g.fold = !HE && T::W == 8 && fabsf(M) <= 128.0f && !(fabsf(g.shift) > 256.0f && b != 0.0f);
+    return g;
+}
+template <class T, bool HE, bool CLAMP>
+__device__ __forceinline__ tok_u4 run_grad(const tok_u4& raw, const RunGrad& g, float c) {
+    float f[T::W], d[T::W];
+    T::unpack(raw, f);
+    if (!HE && T::W == 8 && g.fold) {
+#pragma unroll
+        for (int i = 0; i < T::W; ++i) d[i] = tok_exp2(fmaf(f[i], c, g.shift));
+        tok_u4 r = T::pack(d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] ^= g.sign;
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < T::W; ++i) {
+        const float t = fmaf(f[i], c, -g.M), e = tok_exp2(t);
+        if constexpr (HE) {
+            const float l = fmaf(t, TOK_LN2, g.K);
+            d[i] = e * fmaf(g.hrs, CLAMP ? fmaxf(l, TOK_FAR) : l, g.brs);
+        } else d[i] = e * g.brs;
+    }
+    return T::pack(d);
+}
+template <bool HE>
+__device__ __forceinline__ float run_grad_one(float x, const RunGrad& g, float c) {
+    const float t = fmaf(x, c, -g.M), e = tok_exp2(t);
+    if constexpr (HE) return e * fmaf(g.hrs, fmaxf(fmaf(t, TOK_LN2, g.K), TOK_FAR), g.brs);
+    else return e * g.brs;
+}
+
 // ---------------------------------------------------------------- arguments of every kernel of the family
 enum { TOK_LOGP = 0, TOK_BWD = 1, TOK_POLICY = 2 };
 constexpr int TOK_STATS = CM_NUM_STATS, TOK_MAX_GRID = 2048;
@@ -233,7 +339,7 @@ constexpr int TOK_STATS = CM_NUM_STATS, TOK_MAX_GRID = 2048;
 struct TokArgs {
     const void* logits; int64_t ld; const uint8_t* avail; int64_t avail_ld; const void* token; int token_bytes;
     int64_t rows; int V; TokScale c;
-    float *logp, *entropy; float2* keep;                                     // forward: keep = (m, s), s = 0 for a row that is left out
+    float *logp, *entropy; float2* keep;                                     // forward: keep = (m, s), (M, -s) in the form of TokRun, s = 0 for a row that is left out
     const float2* keep_in; const float *entropy_in, *d_logp, *d_entropy;     // backward
     void* dlogits; int64_t dld;
     const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy

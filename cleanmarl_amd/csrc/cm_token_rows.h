@@ -52,13 +52,37 @@ __device__ __forceinline__ void tok_policy_row(const TokArgs& a, const TokPolicy
     }
 }
 
+// The sums of a row that TokRun cannot form, by the whole workgroup (`sh` is not in use by anyone when this begins)
+template <class T, bool AV, bool EN, int NT>
+__device__ __forceinline__ TokSum tok_careful_sum(const typename T::elem* row, const uint8_t* av, const TokArgs& a, TokSum* sh) {
+    TokSum z = {-FLT_MAX, 0.0f, 0.0f};
+    for (int j = threadIdx.x * T::W; j < a.V; j += NT * T::W) {
+        float f[T::W];
+        tok_load<T, AV>(row, av, j, a.V, f);
+        tok_add<EN>(z, f, a.c.bin);
+    }
+    tok_block<EN, NT / 64>(z, a.c.bin, sh);
+    return z;
+}
+// ... and its gradient, or zeros (g == nullptr)
+template <class T, bool AV, bool EN, int NT>
+__device__ __forceinline__ void tok_careful_grad(const typename T::elem* row, const uint8_t* av, typename T::elem* drow, const TokArgs& a, const TokGrad& g, bool live) {
+    for (int j = threadIdx.x * T::W; j < a.V; j += NT * T::W) {
+        float f[T::W], d[T::W] = {};
+        if (live) {
+            tok_load<T, AV>(row, av, j, a.V, f);
+            tok_grad<EN>(f, j, g, a.c.bin, d);
+        }
+        tok_store<T>(drow, j, a.V, d);
+    }
+}
+
 // Rows that no workgroup can hold: a workgroup walks a row twice, once for (m, s, u) and once, reading it again (a part of it from a cache), to
 // write the gradient.
 template <class T, bool AV, bool EN, int NT>
 __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
     typedef typename T::elem elem;
-    constexpr int W = T::W, NW = NT / 64;
-    __shared__ TokSum sh[2][NW];
+    __shared__ TokSum sh[2][NT / 64];
     double st[TOK_STATS] = {};
     int turn = 0;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -70,14 +94,8 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
         TokGrad g = {};
         float logp = 0.0f;
         if (live) {
-            TokSum z = {-FLT_MAX, 0.0f, 0.0f};
             const float x = tok_logit<T, AV>(row, av, tok, a.V);
-            for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
-                float f[W];
-                tok_load<T, AV>(row, av, j, a.V, f);
-                tok_add<true>(z, f, a.c.bin);
-            }
-            tok_block<true, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+            const TokSum z = tok_careful_sum<T, AV, true, NT>(row, av, a, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
             turn ^= 1;
             live = z.s != 0.0f;
             if (live) {
@@ -92,15 +110,7 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
         }
         if (threadIdx.x == 0 && a.logp) a.logp[r] = logp;
         g.tok = (int)(live && tok < a.V && (!AV || av[tok]) ? tok : -1);  // an unavailable place has no gradient
-        elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
-        for (int j = threadIdx.x * W; j < a.V; j += NT * W) {
-            float f[W], d[W] = {};
-            if (live) {
-                tok_load<T, AV>(row, av, j, a.V, f);
-                tok_grad<EN>(f, j, g, a.c.bin, d);
-            }
-            tok_store<T>(drow, j, a.V, d);
-        }
+        tok_careful_grad<T, AV, EN, NT>(row, av, reinterpret_cast<elem*>(a.dlogits) + r * a.dld, a, g, live);
     }
     if (threadIdx.x == 0)
         for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
@@ -111,7 +121,8 @@ template <class T, bool AV, bool EN, int NT, int U>
 __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, NW = NT / 64;
-    __shared__ TokSum sh[2][NW];
+    __shared__ TokRun sh[2][NW];
+    __shared__ TokSum careful[NW];
     int turn = 0;
     const int nfull = a.V / W, tid = threadIdx.x, jt = nfull * W + tid;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -119,10 +130,11 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
         const int64_t tok = tok_token(a, r);
         const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
         const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
-        TokSum z = {-FLT_MAX, 0.0f, 0.0f};
-        float x = 0.0f;
+        float x = 0.0f, logp = 0.0f, H = 0.0f;
+        float2 keep = {0.0f, 0.0f};
         if (tok >= 0) {
             x = tok_logit<T, AV>(row, av, tok, a.V);
+            TokRun z = {TOK_START, 0.0f, 0.0f};
             tok_u4 raw[U];
             TokAvail<W> ok[AV ? U : 1];
             auto load = [&](int i0) {  // no load depends on a condition: behind the end the row's last piece is read again
@@ -149,19 +161,29 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
 #pragma unroll
                         for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
                     }
-                    tok_add<EN>(z, f, a.c.bin);
+                    run_add<EN, true>(z, f, a.c.bin);
                 }
             }
-            if (jt < a.V && (!AV || av[jt])) { const float one[1] = {T::get(row[jt])}; tok_add<EN, 1>(z, one, a.c.bin); }
-            tok_block<EN, NW>(z, a.c.bin, sh[turn]);
+            if (jt < a.V && (!AV || av[jt])) { const float one[1] = {T::get(row[jt])}; run_add<EN, true>(z, one, a.c.bin); }
+            run_block<EN, NW>(z, sh[turn]);
             turn ^= 1;
+            if (run_ordinary<EN>(z)) {
+                const float logs = logf(z.s);
+                logp = fmaf(x, a.c.bin, -z.M) * TOK_LN2 - logs;
+                H = logs - z.u / z.s * TOK_LN2;
+                keep = make_float2(z.M, -z.s);
+            } else {
+                const TokSum y = tok_careful_sum<T, AV, EN, NT>(row, av, a, careful);
+                const float logs = logf(y.s);
+                if (y.s != 0.0f) { logp = (x - y.m) * a.c.nat - logs; H = logs - y.u / y.s * TOK_LN2; }
+                keep = make_float2(y.m, y.s);
+                __syncthreads();  // `careful` is free again
+            }
         }
         if (tid == 0) {
-            const bool live = z.s != 0.0f;
-            const float logs = logf(z.s);
-            if (a.logp) a.logp[r] = live ? (x - z.m) * a.c.nat - logs : 0.0f;
-            if (EN && a.entropy) a.entropy[r] = live ? logs - z.u / z.s * TOK_LN2 : 0.0f;
-            if (a.keep) a.keep[r] = make_float2(z.m, z.s);
+            if (a.logp) a.logp[r] = logp;
+            if (EN && a.entropy) a.entropy[r] = H;
+            if (a.keep) a.keep[r] = keep;
         }
     }
 }
@@ -192,10 +214,13 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
             continue;
         }
         TokGrad g = {};
-        g.m = keep.x; g.rs = 1.0f / keep.y;
+        const bool run = keep.y < 0.0f;  // the form of TokRun (a sum that is NaN is none)
+        const float s = fabsf(keep.y);
+        g.m = keep.x; g.rs = 1.0f / s;
         g.a = g.b = (tok >= a.V ? NAN : a.d_logp[r]) * a.c.nat;
-        if (EN) { g.K = a.entropy_in[r] - logf(keep.y); g.h = -a.d_entropy[r] * a.c.nat; }
+        if (EN) { g.K = a.entropy_in[r] - logf(s); g.h = -a.d_entropy[r] * a.c.nat; }
         g.tok = (int)(tok < a.V && (!AV || av[tok]) ? tok : -1);
+        const RunGrad gr = run_grad_row<T, EN>(g.m, s, g.K, g.b, g.h);
         tok_u4 raw[U];
         TokAvail<W> ok[AV ? U : 1];
 #pragma unroll
@@ -210,15 +235,34 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
         for (int k = 0; k < U; ++k) {
             const int i = i0 + k * NT + tid;
             if (AV) tok_mask_raw<T>(ok[k], raw[k]);
-            float f[W], d[W];
-            T::unpack(raw[k], f);
-            tok_grad<EN>(f, i * W, g, a.c.bin, d);
-            if (i < nfull) __builtin_nontemporal_store((typename T::vec)T::pack(d), reinterpret_cast<typename T::vec*>(drow) + i);
+            tok_u4 d;
+            if (run) {
+                d = run_grad<T, EN, true>(raw[k], gr, a.c.bin);
+            } else {
+                float f[W], v[W];
+                T::unpack(raw[k], f);
+                tok_grad_rest<EN>(f, g, a.c.bin, v);
+                d = T::pack(v);
+            }
+            if ((unsigned)(g.tok - i * W) < (unsigned)W) {  // the token's own place: from its logit, rounded once
+                float f[W], v[W];
+                T::unpack(raw[k], f);
+                T::unpack(d, v);
+#pragma unroll
+                for (int q = 0; q < W; ++q) {
+                    const float one[1] = {f[q]};
+                    float w[1];
+                    if (run) w[0] = run_grad_one<EN>(f[q], gr, a.c.bin); else tok_grad_rest<EN>(one, g, a.c.bin, w);
+                    if (i * W + q == g.tok) v[q] = w[0] + g.a;
+                }
+                d = T::pack(v);  // the others are what they were
+            }
+            if (i < nfull) __builtin_nontemporal_store((typename T::vec)d, reinterpret_cast<typename T::vec*>(drow) + i);
         }
         if (tail) {
             float d[1];
-            tok_grad<EN>(last, jt, g, a.c.bin, d);
-            drow[jt] = T::put(d[0]);
+            if (run) d[0] = run_grad_one<EN>(last[0], gr, a.c.bin); else tok_grad_rest<EN>(last, g, a.c.bin, d);
+            drow[jt] = T::put(jt == g.tok ? d[0] + g.a : d[0]);
         }
     }
 }
@@ -336,7 +380,8 @@ template <class T, bool AV, bool EN, int NT, int NV, int FULL>
 __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, NW = NT / 64;
-    __shared__ TokSum sh[2][NW];
+    __shared__ TokRun sh[2][NW];
+    __shared__ TokSum careful[NW];
     double st[TOK_STATS] = {};
     int turn = 0;
     const int nfull = a.V / W, tid = threadIdx.x;
@@ -403,67 +448,67 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         bool tok_ok = true;
         if (AV) tok_ok = av[toki] != 0;
         x = tok < a.V ? (tok_ok ? x : -INFINITY) : NAN;
-        TokSum z = {-FLT_MAX, 0.0f, 0.0f};
+        TokRun z = {TOK_START, 0.0f, 0.0f};
         float lastf = -INFINITY;
         if (now.live) {
             lastf = tail && last_ok ? T::get(last) : -INFINITY;
             const float one[1] = {lastf};
-            tok_add<true, 1>(z, one, a.c.bin);
+            run_add<true, true>(z, one, a.c.bin);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 if (k >= FULL && k * NT >= nfull) break;
                 if (AV) tok_mask_raw<T>(ok[k][tid], raw[k]);
                 float f[W];
                 T::unpack(raw[k], f);
-                if (k >= FULL) {
+                if (k < FULL) {
+                    run_add<true, AV>(z, f, a.c.bin);
+                } else {
                     const bool here = tid + k * NT < nfull;
 #pragma unroll
                     for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
+                    run_add<true, true>(z, f, a.c.bin);
                 }
-                tok_add<true>(z, f, a.c.bin);
-                asm volatile("" : "+v"(z.m), "+v"(z.s), "+v"(z.u));  // one piece after the other: interleaved, the floats of all of them would be live at once
+                asm volatile("" : "+v"(z.M), "+v"(z.s), "+v"(z.u));  // one piece after the other: interleaved, the floats of all of them would be live at once
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (AV) {
 #pragma unroll
                 for (int k = 0; k < R; ++k) ring[k] = piece_av(nav, k);
             }
-            tok_block<true, NW>(z, a.c.bin, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
+            run_block<true, NW>(z, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
             turn ^= 1;
         }
-        const bool live = now.live && z.s != 0.0f;
+        const bool ordinary = run_ordinary<true>(z);
+        TokSum y = {0.0f, 0.0f, 0.0f};
+        if (now.live && !ordinary) { y = tok_careful_sum<T, AV, true, NT>(row, av, a, careful); __syncthreads(); }
+        const float s = ordinary ? z.s : y.s;
+        const bool live = now.live && s != 0.0f;
         TokGrad g = {};  // all zero: a row that is left out gets zeros
+        RunGrad gr = {};
         float logp = 0.0f, H = 0.0f;
         if (live) {
-            const float logs = logf(z.s);
-            g.m = z.m; g.rs = 1.0f / z.s;
-            logp = (x - z.m) * a.c.nat - logs;
-            g.K = -z.u * g.rs * TOK_LN2; H = logs + g.K;
+            const float logs = logf(s);
+            g.m = y.m; g.rs = 1.0f / s;
+            logp = (ordinary ? fmaf(x, a.c.bin, -z.M) * TOK_LN2 : (x - y.m) * a.c.nat) - logs;
+            g.K = -(ordinary ? z.u : y.u) * g.rs * TOK_LN2; H = logs + g.K;
             float gg, hh;
             tok_policy_row(a, now.q, logp, H, tid == 0, st, gg, hh);
             g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
+            if (ordinary) gr = run_grad_row<T, EN>(z.M, s, g.K, g.b, g.h);
         }
         if (tid == 0 && a.logp) a.logp[r] = logp;
         {
             g.tok = live && tok < a.V && tok_ok ? toki : -1;
             elem* drow = reinterpret_cast<elem*>(a.dlogits) + r * a.dld;
-            if (now.live) {
-                if (tail) {
-                    float d[1];
-                    const float f[1] = {lastf};
-                    tok_grad_rest<EN>(f, g, a.c.bin, d);
-                    drow[jt] = T::put(d[0]);
-                }
+            if (now.live && ordinary) {
+                if (tail) drow[jt] = T::put(run_grad_one<EN>(lastf, gr, a.c.bin));
                 last = nrow[jt];
                 if (AV) last_ok = nav[jt];
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     asm volatile("" : "+v"(raw[k]));  // unpacked again: the floats of the first sweep would be kept, at two registers for one
                     if (k < FULL || tid + k * NT < nfull) {
-                        float f[W], d[W];
-                        T::unpack(raw[k], f);
-                        tok_grad_rest<EN>(f, g, a.c.bin, d);
-                        __builtin_nontemporal_store((typename T::vec)T::pack(d), at(drow, k));
+                        __builtin_nontemporal_store((typename T::vec)run_grad<T, EN, AV>(raw[k], gr, a.c.bin), at(drow, k));
                     }
                     if (AV) {
                         ok[k][tid] = ring[k % R];
@@ -474,18 +519,13 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
                 }
                 // the token's place once more, by the thread that has just written it: a comparison in every piece would be a branch in every piece
                 if (g.tok >= 0 && tid == (g.tok < nfull * W ? (g.tok / W) & (NT - 1) : g.tok - nfull * W)) {
-                    const float f[1] = {x};
-                    float d[1];
-                    tok_grad_rest<EN>(f, g, a.c.bin, d);
-                    drow[g.tok] = T::put(d[0] + g.a);
+                    drow[g.tok] = T::put(run_grad_one<EN>(x, gr, a.c.bin) + g.a);
                 }
-            } else {
-                if (tail) drow[jt] = T::put(0.0f);
-#pragma unroll
-                for (int k = 0; k < NV; ++k) if (k < FULL || tid + k * NT < nfull) *at(drow, k) = tok_u4{0u, 0u, 0u, 0u};
+            } else {  // zeros, or the careful form from memory; the next row replaces what the registers hold
+                tok_careful_grad<T, AV, EN, NT>(row, av, drow, a, g, live);
+                fill(nrow, nav);
             }
         }
-        if (!now.live) fill(nrow, nav);  // nothing has been used up: the next row replaces what is there
         now = next;
     }
     if (tid == 0)
