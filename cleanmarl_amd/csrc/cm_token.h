@@ -128,6 +128,22 @@ __device__ __forceinline__ void tok_load(const typename T::elem* row, const uint
     T::unpack(tok_raw<T>(row, j, V), f);
     if constexpr (AV) tok_mask<T::W>(tok_raw_avail<T::W>(av, j, V), f);
 }
+// A long row is taken apart into a body of whole pieces that begin on a cache line (where a row of an odd vocabulary does not: pieces
+// across lines cost a sixth of the bandwidth) and at most 127 bytes in front and 15 behind it, which the first threads take one element each.
+struct TokShape {
+    int head, full, edges;  // elements in front of the body, pieces in it, elements outside it
+    __device__ __forceinline__ int edge(int t, int W) const { return t < head ? t : full * W + t; }                              // element of thread t < edges
+    __device__ __forceinline__ int piece(int j, int W) const { return j < head || j >= head + full * W ? -1 : (j - head) / W; }  // piece of element j, -1: an edge
+    __device__ __forceinline__ int edge_of(int j, int W) const { return j < head ? j : j - full * W; }
+};
+template <class T>
+__device__ __forceinline__ TokShape tok_shape(const typename T::elem* row, int V, unsigned peel) {  // peel: 127, or 0 for none
+    TokShape s;
+    s.head = (int)((-(unsigned)reinterpret_cast<uintptr_t>(row) & peel) / sizeof(typename T::elem));
+    s.full = (V - s.head) / T::W;
+    s.edges = V - s.full * T::W;
+    return s;
+}
 template <class T>
 __device__ __forceinline__ void tok_store(typename T::elem* row, int j, int V, const float (&f)[T::W]) {
     constexpr int W = T::W;
@@ -343,9 +359,13 @@ struct TokArgs {
     const float2* keep_in; const float *entropy_in, *d_logp, *d_entropy;     // backward
     void* dlogits; int64_t dld;
     const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy
+    const int32_t* order; unsigned peel;                                      // long rows: the order in which they are taken, NULL: as they are
     const int32_t* range_lo; const int32_t* range_hi;                        // preference: only the rows [*range_lo, *range_hi) are touched
 };
-// launches the kernels of one type; returns the number of partial rows of statistics (TOK_POLICY)
-int tok_launch_f32(const TokArgs& a, int mode, bool en, hipStream_t s);
-int tok_launch_f16(const TokArgs& a, int mode, bool en, hipStream_t s);
-int tok_launch_bf16(const TokArgs& a, int mode, bool en, hipStream_t s);
+constexpr int TOK_ORDER_ROWS = 1 << 20;  // the most rows that are put in order
+// (rows that count first, the others behind them: cm_token.hip)
+int tok_launch_order(const TokArgs& a, int32_t* order, hipStream_t s);
+// launches the kernels of one type; `scratch`: room for an order; returns the number of partial rows of statistics (TOK_POLICY)
+int tok_launch_f32(TokArgs a, int mode, bool en, int32_t* scratch, hipStream_t s);
+int tok_launch_f16(TokArgs a, int mode, bool en, int32_t* scratch, hipStream_t s);
+int tok_launch_bf16(TokArgs a, int mode, bool en, int32_t* scratch, hipStream_t s);

@@ -25,6 +25,29 @@ __global__ __launch_bounds__(256) void k_tok_stats(const double* __restrict__ pa
     }
 }
 
+// order[0 .. n): the rows that count, in their order, then the others.  One workgroup; a thread counts and places a run of rows.
+__global__ __launch_bounds__(1024) void k_tok_order(const void* __restrict__ token, int token_bytes, const float* __restrict__ weight, int rows, int32_t* __restrict__ order) {
+    __shared__ int waves[16];
+    const int per = (rows + 1023) / 1024, b = min((int)threadIdx.x * per, rows), e = min(b + per, rows);
+    auto counts = [&](int r) {
+        const bool there = token_bytes == 8 ? reinterpret_cast<const int64_t*>(token)[r] >= 0 : reinterpret_cast<const int32_t*>(token)[r] >= 0;
+        return there && (!weight || weight[r] != 0.0f);
+    };
+    int mine = 0;
+    for (int r = b; r < e; ++r) mine += counts(r) ? 1 : 0;
+    int upto = mine;  // of this thread and those before it in the wave
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(upto, o, 64); if ((int)(threadIdx.x & 63) >= o) upto += v; }
+    if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    int before = upto - mine, total = 0;
+    for (int w = 0; w < 16; ++w) { if (w < (int)(threadIdx.x >> 6)) before += waves[w]; total += waves[w]; }
+    for (int r = b; r < e; ++r) {
+        if (counts(r)) order[before++] = r;
+        else order[total + r - before] = r;  // `before` of the rows in front of r count
+    }
+}
+
 // One workgroup per pair: log-probabilities of its two sequences (64-bit sums: thousands of terms, and only their difference counts),
 // the margin, the loss and the factor that every row of the two sequences gets.
 struct PrefArgs {
@@ -76,13 +99,14 @@ __global__ __launch_bounds__(256) void k_pref_pair(const PrefArgs a) {
 }
 
 // ---------------------------------------------------------------- host side
-int tok_launch(const TokArgs& a, int dtype, int mode, bool en, hipStream_t s) {  // the number of partial rows of statistics
+int tok_launch(const TokArgs& a, int dtype, int mode, bool en, int32_t* scratch, hipStream_t s) {  // the number of partial rows of statistics
     if (a.rows == 0) return 0;
-    return dtype == CM_DTYPE_F32 ? tok_launch_f32(a, mode, en, s) : dtype == CM_DTYPE_F16 ? tok_launch_f16(a, mode, en, s) : tok_launch_bf16(a, mode, en, s);
+    return dtype == CM_DTYPE_F32 ? tok_launch_f32(a, mode, en, scratch, s) : dtype == CM_DTYPE_F16 ? tok_launch_f16(a, mode, en, scratch, s) : tok_launch_bf16(a, mode, en, scratch, s);
 }
 
 inline size_t tok_elem(int dtype) { return dtype == CM_DTYPE_F32 ? 4 : 2; }
-inline size_t tok_up(size_t n) { return (n + 255) & ~(size_t)255; }
+constexpr size_t tok_up(size_t n) { return (n + 255) & ~(size_t)255; }
+constexpr size_t TOK_PART_BYTES = (size_t)TOK_MAX_GRID * TOK_STATS * sizeof(double);
 
 int tok_check(const char* who, const cm_token_rows_t* t) {
     CM_REQUIRE(t, "%s: NULL cm_token_rows_t", who);
@@ -121,9 +145,14 @@ TokArgs tok_args(const cm_token_rows_t* t) {
 
 }  // namespace
 
+int tok_launch_order(const TokArgs& a, int32_t* order, hipStream_t s) {
+    hipLaunchKernelGGL(k_tok_order, dim3(1), dim3(1024), 0, s, a.token, a.token_bytes, a.weight, (int)a.rows, order);
+    return 0;
+}
+
 extern "C" size_t cm_token_workspace_bytes(int64_t rows, int vocab) {
     if (rows < 0 || vocab < 1) return 0;
-    return tok_up((size_t)TOK_MAX_GRID * TOK_STATS * sizeof(double));
+    return TOK_PART_BYTES + tok_up((size_t)(rows < TOK_ORDER_ROWS ? rows : TOK_ORDER_ROWS) * sizeof(int32_t));
 }
 
 extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* entropy, float* keep, void* ws, size_t ws_bytes, cm_stream_t stream) {
@@ -134,7 +163,7 @@ extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* en
     CM_REQUIRE(ws && ws_bytes >= need, "cm_token_logprob: workspace too small (%zu < %zu)", ws_bytes, need);
     TokArgs a = tok_args(t);
     a.logp = logp; a.entropy = entropy; a.keep = (float2*)keep;
-    tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, (hipStream_t)stream);
+    tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, nullptr, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_logprob");
     return 0;
 }
@@ -148,7 +177,7 @@ extern "C" int cm_token_logprob_bwd(const cm_token_rows_t* t, const float* keep,
     CM_REQUIRE(reinterpret_cast<uintptr_t>(keep) % 8 == 0, "cm_token_logprob_bwd: keep must be 8-byte aligned");
     TokArgs a = tok_args(t);
     a.keep_in = (const float2*)keep; a.entropy_in = entropy; a.d_logp = d_logp; a.d_entropy = d_entropy; a.dlogits = dlogits; a.dld = dlogits_ld;
-    tok_launch(a, t->dtype, TOK_BWD, d_entropy != nullptr, (hipStream_t)stream);
+    tok_launch(a, t->dtype, TOK_BWD, d_entropy != nullptr, nullptr, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_logprob_bwd");
     return 0;
 }
@@ -168,7 +197,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
     a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws;
-    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, (hipStream_t)stream);
+    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, (int32_t*)((char*)ws + TOK_PART_BYTES), (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd");
     hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(256), 0, (hipStream_t)stream, a.part, parts, stats);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd/stats");
@@ -203,13 +232,13 @@ extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* se
     hipStream_t s = (hipStream_t)stream;
     TokArgs a = tok_args(t);
     a.range_lo = seq_start; a.range_hi = seq_start + 2 * pairs; a.logp = logp; a.keep = keep;
-    tok_launch(a, t->dtype, TOK_LOGP, false, s);
+    tok_launch(a, t->dtype, TOK_LOGP, false, nullptr, s);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/logp");
     PrefArgs p = {logp, seq_start, pairs, t->rows, logp_ref, beta, label_smoothing, scale, kind, coef, margin, seq_logp, part};
     hipLaunchKernelGGL(k_pref_pair, dim3(pairs), dim3(256), 0, s, p);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/pair");
     a.keep_in = keep; a.d_logp = coef; a.dlogits = dlogits; a.dld = dlogits_ld;
-    tok_launch(a, t->dtype, TOK_BWD, false, s);
+    tok_launch(a, t->dtype, TOK_BWD, false, nullptr, s);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/bwd");
     hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(256), 0, s, part, pairs, stats);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/stats");

@@ -518,7 +518,7 @@ int cm_polyak_update(float* target, const float* src, int64_t n, double polyak, 
  * its weight is 0 or none of its columns is available (every logit -inf counts as that); the logits of a row that is left out for its
  * token or weight are not read.  A token >= vocab gives NaN.  The gradient has the logits' type, is rounded once, and may be
  * written over the logits (dlogits == logits with the same row stride); any other overlap is refused.  Per-row vectors are fp32 and contiguous.
- * All sums are formed in a fixed order: the same inputs give the same bits. */
+ * All sums are formed in a fixed order, which may depend on the alignment of the rows: the same inputs at equal alignments give the same bits. */
 enum { CM_DTYPE_F32 = 0, CM_DTYPE_F16 = 1, CM_DTYPE_BF16 = 2 };
 typedef struct cm_token_rows {
     const void* logits;      /* [rows][vocab], row stride ld (elements); aligned to the element only */

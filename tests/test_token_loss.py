@@ -207,7 +207,8 @@ def test_logprob_forward_and_backward(rows, V, dtype):
             assert bool((got.cpu()[mask.cpu() == 0] == 0).all())
         y = x.clone() if pad == 0 else x  # in place: over the logits' own rows, whatever their stride
         out = TL.token_logprob_bwd(y, tok, r, dl.cuda(), d_entropy=dh.cuda() if entropy else None, avail=mask, temperature=T, out=y)
-        assert out.data_ptr() == y.data_ptr() and torch.equal(out, got)
+        assert out.data_ptr() == y.data_ptr()
+        close(out, want, bar, "dlogits in place")  # (another address may take a row apart differently: the bits are those of an equal alignment)
 
 
 @pytest.mark.gpu
@@ -337,15 +338,21 @@ def test_policy_loss(rows, V, dtype):
         err_row = dict(zip(range(8), [whole * (delta + 6 * U), want["w"] * bars.H, want["w"] * (want["rho"] * (delta + 4 * U) + delta + 4 * U), 0 * whole,
                                       whole * (delta + 8 * U) + want["w"] * (ent * bars.H + 8 * U) + ek * (delta + 4 * U) + kl * want["w"] * (delta + 4 * U), 0 * whole,
                                       want["w"] * ((want["kl"] + 2) * 2 * (delta + 4 * U)) if kl else 0 * whole, 0 * whole]))
-        for i in range(8):
-            v = want["rows"][i] if i == 5 else want["rows"][i] * want["w"]
-            v = torch.where(live, v, 0.0)
-            bar_i = float(torch.where(live, err_row[i] + 4 * U * v.abs(), 0.0).sum()) + 2 * U * abs(float(v.sum()))
-            assert abs(float(r.stats[i]) - float(v.sum())) <= bar_i, (i, float(r.stats[i]), float(v.sum()), bar_i)
-        again = TL.policy_loss_fwd_bwd(x, tok, cu(old), cu(adv), logp_ref=cu(refp), weight=cu(w), avail=mask, temperature=T, clip_low=lo, clip_high=hi, kl_coef=kl, entropy_coef=ent)
+
+        def check_stats(stats):
+            for i in range(8):
+                v = want["rows"][i] if i == 5 else want["rows"][i] * want["w"]
+                v = torch.where(live, v, 0.0)
+                bar_i = float(torch.where(live, err_row[i] + 4 * U * v.abs(), 0.0).sum()) + 2 * U * abs(float(v.sum()))
+                assert abs(float(stats[i]) - float(v.sum())) <= bar_i, (i, float(stats[i]), float(v.sum()), bar_i)
+
+        check_stats(r.stats)
+        args = dict(logp_ref=cu(refp), weight=cu(w), avail=mask, temperature=T, clip_low=lo, clip_high=hi, kl_coef=kl, entropy_coef=ent)
+        again = TL.policy_loss_fwd_bwd(x, tok, cu(old), cu(adv), **args)
         assert torch.equal(again.stats, r.stats) and torch.equal(again.dlogits, r.dlogits)  # the same bits every time
-        over = TL.policy_loss_fwd_bwd(x, tok, cu(old), cu(adv), logp_ref=cu(refp), weight=cu(w), avail=mask, temperature=T, clip_low=lo, clip_high=hi, kl_coef=kl, entropy_coef=ent, out=x)
-        assert torch.equal(over.dlogits, r.dlogits) and torch.equal(over.stats, r.stats)
+        over = TL.policy_loss_fwd_bwd(x, tok, cu(old), cu(adv), out=x, **args)
+        close(over.dlogits, dwant, bar, "dlogits in place")
+        check_stats(over.stats)
 
 
 @pytest.mark.gpu
