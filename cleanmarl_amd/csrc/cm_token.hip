@@ -29,12 +29,20 @@ __global__ __launch_bounds__(256) void k_tok_stats(const double* __restrict__ pa
 __global__ __launch_bounds__(1024) void k_tok_order(const void* __restrict__ token, int token_bytes, const float* __restrict__ weight, int rows, int32_t* __restrict__ order) {
     __shared__ int waves[16];
     const int per = (rows + 1023) / 1024, b = min((int)threadIdx.x * per, rows), e = min(b + per, rows);
+    const int32_t* sign = reinterpret_cast<const int32_t*>(token) + (token_bytes == 8 ? 1 : 0);  // the word that holds it
     auto counts = [&](int r) {
-        const bool there = token_bytes == 8 ? reinterpret_cast<const int64_t*>(token)[r] >= 0 : reinterpret_cast<const int32_t*>(token)[r] >= 0;
-        return there && (!weight || weight[r] != 0.0f);
+        const int32_t t = sign[(int64_t)r * (token_bytes / 4)];
+        const float w = weight ? weight[r] : 1.0f;
+        return (t >= 0) & (w != 0.0f);
+    };
+    auto eight = [&](int r0) {  // which of the rows r0 .. r0 + 7 count: their loads are in flight together
+        unsigned bits = 0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { const int r = min(r0 + q, rows - 1); bits |= (r0 + q < e && counts(r) ? 1u : 0u) << q; }
+        return bits;
     };
     int mine = 0;
-    for (int r = b; r < e; ++r) mine += counts(r) ? 1 : 0;
+    for (int r = b; r < e; r += 8) mine += __popc(eight(r));
     int upto = mine;  // of this thread and those before it in the wave
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(upto, o, 64); if ((int)(threadIdx.x & 63) >= o) upto += v; }
@@ -42,9 +50,12 @@ __global__ __launch_bounds__(1024) void k_tok_order(const void* __restrict__ tok
     __syncthreads();
     int before = upto - mine, total = 0;
     for (int w = 0; w < 16; ++w) { if (w < (int)(threadIdx.x >> 6)) before += waves[w]; total += waves[w]; }
-    for (int r = b; r < e; ++r) {
-        if (counts(r)) order[before++] = r;
-        else order[total + r - before] = r;  // `before` of the rows in front of r count
+    for (int r0 = b; r0 < e; r0 += 8) {
+        const unsigned bits = eight(r0);
+        for (int q = 0; q < 8 && r0 + q < e; ++q) {
+            if (bits >> q & 1u) order[before++] = r0 + q;
+            else order[total + r0 + q - before] = r0 + q;  // `before` of the rows in front of it count
+        }
     }
 }
 
@@ -99,7 +110,7 @@ __global__ __launch_bounds__(256) void k_pref_pair(const PrefArgs a) {
 }
 
 // ---------------------------------------------------------------- host side
-int tok_launch(const TokArgs& a, int dtype, int mode, bool en, int32_t* scratch, hipStream_t s) {  // the number of partial rows of statistics
+int tok_launch(const TokArgs& a, int dtype, int mode, bool en, void* scratch, hipStream_t s) {  // the number of partial rows of statistics
     if (a.rows == 0) return 0;
     return dtype == CM_DTYPE_F32 ? tok_launch_f32(a, mode, en, scratch, s) : dtype == CM_DTYPE_F16 ? tok_launch_f16(a, mode, en, scratch, s) : tok_launch_bf16(a, mode, en, scratch, s);
 }
@@ -108,6 +119,9 @@ inline size_t tok_elem(int dtype) { return dtype == CM_DTYPE_F32 ? 4 : 2; }
 constexpr size_t tok_up(size_t n) { return (n + 255) & ~(size_t)255; }
 constexpr size_t TOK_PART_BYTES = (size_t)TOK_MAX_GRID * TOK_STATS * sizeof(double);
 
+size_t tok_scratch(int64_t rows) {  // an order of many rows or the partial sums of few
+    return rows <= TOK_SPLIT_ROWS ? tok_up(TOK_SPLIT_BYTES) : rows <= TOK_ORDER_ROWS ? tok_up((size_t)rows * sizeof(int32_t)) : 0;
+}
 int tok_check(const char* who, const cm_token_rows_t* t) {
     CM_REQUIRE(t, "%s: NULL cm_token_rows_t", who);
     CM_REQUIRE(t->dtype == CM_DTYPE_F32 || t->dtype == CM_DTYPE_F16 || t->dtype == CM_DTYPE_BF16, "%s: unknown dtype %d", who, (int)t->dtype);
@@ -152,7 +166,7 @@ int tok_launch_order(const TokArgs& a, int32_t* order, hipStream_t s) {
 
 extern "C" size_t cm_token_workspace_bytes(int64_t rows, int vocab) {
     if (rows < 0 || vocab < 1) return 0;
-    return TOK_PART_BYTES + tok_up((size_t)(rows < TOK_ORDER_ROWS ? rows : TOK_ORDER_ROWS) * sizeof(int32_t));
+    return TOK_PART_BYTES + tok_scratch(rows);
 }
 
 extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* entropy, float* keep, void* ws, size_t ws_bytes, cm_stream_t stream) {
@@ -160,10 +174,10 @@ extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* en
     CM_REQUIRE(t->rows == 0 || logp, "cm_token_logprob: NULL logp");
     CM_REQUIRE(reinterpret_cast<uintptr_t>(keep) % 8 == 0, "cm_token_logprob: keep must be 8-byte aligned");
     const size_t need = cm_token_workspace_bytes(t->rows, t->vocab);
-    CM_REQUIRE(ws && ws_bytes >= need, "cm_token_logprob: workspace too small (%zu < %zu)", ws_bytes, need);
+    CM_REQUIRE(ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "cm_token_logprob: workspace too small (%zu < %zu) or not 16-byte aligned", ws_bytes, need);
     TokArgs a = tok_args(t);
     a.logp = logp; a.entropy = entropy; a.keep = (float2*)keep;
-    tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, nullptr, (hipStream_t)stream);
+    tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, (char*)ws + TOK_PART_BYTES, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_logprob");
     return 0;
 }
@@ -197,7 +211,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
     a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws;
-    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, (int32_t*)((char*)ws + TOK_PART_BYTES), (hipStream_t)stream);
+    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, (char*)ws + TOK_PART_BYTES, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd");
     hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(256), 0, (hipStream_t)stream, a.part, parts, stats);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd/stats");
@@ -207,7 +221,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
 extern "C" size_t cm_preference_workspace_bytes(int64_t rows, int vocab, int pairs) {
     if (rows < 0 || vocab < 1 || pairs < 1) return 0;
     return tok_up((size_t)rows * sizeof(float2)) + 2 * tok_up((size_t)rows * sizeof(float)) +
-           tok_up((size_t)pairs * TOK_STATS * sizeof(double));
+           tok_up((size_t)pairs * TOK_STATS * sizeof(double)) + tok_scratch(rows);
 }
 
 extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* seq_start, int pairs, const float* logp_ref, double beta,
@@ -228,11 +242,11 @@ extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* se
     float2* keep = (float2*)w; w += tok_up((size_t)t->rows * sizeof(float2));
     float* logp = (float*)w; w += tok_up((size_t)t->rows * sizeof(float));
     float* coef = (float*)w; w += tok_up((size_t)t->rows * sizeof(float));
-    double* part = (double*)w;
+    double* part = (double*)w; w += tok_up((size_t)pairs * TOK_STATS * sizeof(double));
     hipStream_t s = (hipStream_t)stream;
     TokArgs a = tok_args(t);
     a.range_lo = seq_start; a.range_hi = seq_start + 2 * pairs; a.logp = logp; a.keep = keep;
-    tok_launch(a, t->dtype, TOK_LOGP, false, nullptr, s);
+    tok_launch(a, t->dtype, TOK_LOGP, false, w, s);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/logp");
     PrefArgs p = {logp, seq_start, pairs, t->rows, logp_ref, beta, label_smoothing, scale, kind, coef, margin, seq_logp, part};
     hipLaunchKernelGGL(k_pref_pair, dim3(pairs), dim3(256), 0, s, p);

@@ -193,6 +193,106 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
     }
 }
 
+// Few long rows: a row is cut into segments, a workgroup sums one, k_tok_join puts them together.  (16 rows of 131072 bf16 columns: 13.3 us with
+// a workgroup per row.)
+template <class T, bool AV, bool EN, int NT>
+__global__ __launch_bounds__(NT) void k_tok_part(const TokArgs a) {
+    typedef typename T::elem elem;
+    constexpr int W = T::W, NW = NT / 64;
+    __shared__ TokRun sh[NW];
+    const int tid = threadIdx.x, seg = blockIdx.x;
+    const int64_t r = blockIdx.y;
+    const int64_t tok = tok_in_range(a, r) ? tok_token(a, r) : -1;
+    if (tok < 0 || (a.weight && a.weight[r] == 0.0f)) return;  // k_tok_join does not look at it either
+    const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
+    const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
+    const TokShape shape = tok_shape<T>(row, a.V, a.peel);
+    const elem* body = row + shape.head;
+    const int len = (shape.full + a.segs - 1) / a.segs, b = seg * len, e = min(b + len, shape.full);
+    TokRun z = {TOK_START, 0.0f, 0.0f};
+    for (int i = b + tid; i < e; i += NT) {
+        tok_u4 raw = reinterpret_cast<const typename T::vec*>(body)[i];
+        if (AV) tok_mask_raw<T>(tok_avail<W>(av + shape.head, i * W), raw);
+        float f[W];
+        T::unpack(raw, f);
+        run_add<EN, true>(z, f, a.c.bin);
+    }
+    const int je = shape.edge(tid, W);
+    if (seg == 0 && tid < shape.edges && (!AV || av[je])) { const float one[1] = {T::get(row[je])}; run_add<EN, true>(z, one, a.c.bin); }
+    run_block<EN, NW>(z, sh);
+    if (tid == 0) a.split[r * a.segs + seg] = make_float4(z.M, z.s, z.u, seg == 0 ? tok_logit<T, AV>(row, av, tok, a.V) : 0.0f);
+}
+
+// Half a wave per row and round.  TOK_POLICY: one workgroup, which adds up the statistics as well and leaves to k_tok_back what it needs of each row.
+template <class T, int MODE, bool AV, bool EN, int NT>
+__global__ __launch_bounds__(NT) void k_tok_join(const TokArgs a) {
+    typedef typename T::elem elem;
+    constexpr int PER = NT / 32;
+    constexpr bool ENT = EN || MODE == TOK_POLICY;
+    __shared__ TokSum careful[NT / 64], sums[PER];
+    __shared__ int odd[PER];
+    __shared__ double sh[NT / 64][TOK_STATS];
+    const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
+    double st[TOK_STATS] = {};
+    for (int64_t r0 = (int64_t)blockIdx.x * PER; r0 < a.rows; r0 += (int64_t)gridDim.x * PER) {
+        const int64_t r = r0 + slot;
+        const bool here = r < a.rows && tok_in_range(a, r);
+        const int64_t tok = here ? tok_token(a, r) : -1;
+        TokPolicyRow q = {};
+        if (MODE == TOK_POLICY && here) q = tok_policy_load(a, r);
+        const bool counts = tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f);
+        TokRun z = {TOK_START, 0.0f, 0.0f};
+        float x = 0.0f;
+        if (counts) {
+            const float4 v = lane < a.segs ? a.split[r * a.segs + lane] : make_float4(TOK_START, 0.0f, 0.0f, 0.0f);
+            z = {v.x, v.y, v.z};
+            x = __shfl(v.w, threadIdx.x & 32, 64);
+            run_group<ENT, 32>(z);
+        }
+        const bool ordinary = run_ordinary<ENT>(z);
+        if (lane == 0) odd[slot] = counts && !ordinary;
+        __syncthreads();
+        for (int p = 0; p < PER; ++p) {  // rows that have to be done over, by all
+            if (!odd[p]) continue;
+            const TokSum y = tok_careful_sum<T, AV, ENT, NT>(reinterpret_cast<const elem*>(a.logits) + (r0 + p) * a.ld, AV ? a.avail + (r0 + p) * a.avail_ld : nullptr, a, careful);
+            if (threadIdx.x == 0) sums[p] = y;
+            __syncthreads();
+        }
+        if (here && lane == 0) {
+            float logp = 0.0f, H = 0.0f, g = 0.0f, h = 0.0f;
+            float2 keep = {0.0f, 0.0f};
+            if (counts) {
+                const TokSum y = ordinary ? TokSum{0.0f, z.s, z.u} : sums[slot];
+                const float logs = logf(y.s);
+                if (y.s != 0.0f) {
+                    logp = (ordinary ? fmaf(x, a.c.bin, -z.M) * TOK_LN2 : (x - y.m) * a.c.nat) - logs;
+                    if (ENT) H = logs - y.u / y.s * TOK_LN2;
+                    if (MODE == TOK_POLICY) tok_policy_row(a, q, logp, H, true, st, g, h);
+                }
+                keep = ordinary ? make_float2(z.M, -z.s) : make_float2(y.m, y.s);
+            }
+            if (a.logp) a.logp[r] = logp;
+            if (a.keep) a.keep[r] = keep;
+            if (ENT && a.entropy) a.entropy[r] = H;
+            if (MODE == TOK_POLICY) { a.g_out[r] = g; a.h_out[r] = -h; }
+        }
+        __syncthreads();  // odd, sums, careful are free again
+    }
+    if (MODE == TOK_POLICY) {
+#pragma unroll
+        for (int i = 0; i < TOK_STATS; ++i) {
+            const double v = cm_wave_sum_d(st[i]);
+            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6][i] = v;
+        }
+        __syncthreads();
+        if (threadIdx.x < TOK_STATS) {
+            double v = 0.0;
+            for (int w = 0; w < NT / 64; ++w) v += sh[w][threadIdx.x];
+            a.part[threadIdx.x] = v;
+        }
+    }
+}
+
 // Backward only, rows too long for a wave: nothing is summed, so a workgroup takes NT * U pieces of one row, whichever.  The rows come in
 // descending order: the last ones that a forward sweep has read are the ones still in a cache.
 template <class T, bool AV, bool EN, int NT, int U>
@@ -559,7 +659,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
 inline int tok_grid(int64_t items) { return (int)(items < TOK_MAX_GRID ? (items < 1 ? 1 : items) : TOK_MAX_GRID); }
 
 template <class T, int MODE, bool AV, bool EN>
-int tok_launch4(TokArgs& a, int32_t* scratch, hipStream_t s) {
+int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
     const int64_t nvec = ((int64_t)a.V + T::W - 1) / T::W;
 #define TOK_SHORT(G, NV) do { const int grid = tok_grid((a.rows + 256 / G - 1) / (256 / G)); \
         hipLaunchKernelGGL((k_tok_short<T, MODE, AV, EN, G, NV>), dim3(grid), dim3(256), 0, s, a); return grid; } while (0)
@@ -568,28 +668,57 @@ int tok_launch4(TokArgs& a, int32_t* scratch, hipStream_t s) {
     if (nvec <= 32) TOK_SHORT(16, 2);
     if (nvec <= 128) TOK_SHORT(64, 2);
 #undef TOK_SHORT
-    if constexpr (MODE == TOK_BWD) {
+    const int64_t nfull = a.V / T::W;
+    auto back = [&](const TokArgs& b) {
         constexpr int NT = 256, U = 4;
-        a.peel = 127u;
-        const int parts = (int)((a.V / T::W + NT * U - 1) / (NT * U));
-        const int64_t tiles = a.rows * parts;
-        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, a, parts, tiles);
+        const int parts = (int)((nfull + NT * U - 1) / (NT * U));
+        const int64_t tiles = b.rows * parts;
+        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, b, parts, tiles);
+    };
+    a.peel = 127u;
+    if constexpr (MODE == TOK_BWD) {
+        back(a);
         return 0;
     }
-    if constexpr (MODE == TOK_LOGP) {
+    // few long rows: enough segments for some 1024 workgroups, at least 512 pieces (8 KB) in each
+    const int64_t most = 1024 / a.rows < nfull / 512 ? 1024 / a.rows : nfull / 512;
+    a.segs = (int)(most < TOK_SPLIT_SEGS ? most : TOK_SPLIT_SEGS);
+    const bool split = scratch && a.rows <= TOK_SPLIT_ROWS && a.segs >= 2;
+    if (split) {
+        a.split = reinterpret_cast<float4*>(scratch);
         a.peel = 127u;
+    }
+    if constexpr (MODE == TOK_LOGP) {
+        if (split) {
+            hipLaunchKernelGGL((k_tok_part<T, AV, EN, 256>), dim3(a.segs, (unsigned)a.rows), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_tok_join<T, MODE, AV, EN, 256>), dim3((unsigned)(a.rows + 7) / 8), dim3(256), 0, s, a);
+            return 0;
+        }
         const int grid = (int)(a.rows < (1 << 20) ? a.rows : (1 << 20));
         hipLaunchKernelGGL((k_tok_sum<T, AV, EN, 256, 2>), dim3(grid), dim3(256), 0, s, a);
         return grid;
     }
     if constexpr (MODE == TOK_POLICY) {
-        const int64_t nfull = a.V / T::W;
+        // a third launch instead of one sweep of whole rows: from rows on that keep a workgroup busy for some 10 us
+        if (split && a.rows <= 64 && nfull > 512 * 12) {
+            a.keep = reinterpret_cast<float2*>(a.split + TOK_SPLIT_ROWS * TOK_SPLIT_SEGS);
+            a.g_out = reinterpret_cast<float*>(a.keep + TOK_SPLIT_ROWS); a.h_out = a.g_out + TOK_SPLIT_ROWS; a.entropy = a.h_out + TOK_SPLIT_ROWS;
+            hipLaunchKernelGGL((k_tok_part<T, AV, true, 256>), dim3(a.segs, (unsigned)a.rows), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_tok_join<T, MODE, AV, EN, 1024>), dim3(1), dim3(1024), 0, s, a);
+            TokArgs b = a;
+            b.keep_in = a.keep; b.entropy_in = a.entropy; b.d_logp = a.g_out; b.d_entropy = a.h_out;
+            back(b);
+            return 1;
+        }
         constexpr int HEAD = (128 / (int)sizeof(typename T::elem) + T::W - 1) / T::W;  // the most pieces that a head takes from the body
         // FULL pieces of every thread exist: nfull > NT * FULL; a head is only peeled off where they still do
         // Rows that are left out (prompts, padding) cost next to nothing and come in patterns: without an order some workgroups would get few of
         // them (3001 x 100003 fp16, 30 % left out: 430 -> 330 us).  The order costs a launch and 5 us for 8192 rows: worth it from some 50 us on.
         auto in_order = [&](int grid) {
-            if (scratch && a.rows > grid && a.rows <= TOK_ORDER_ROWS && a.rows * a.V >= (int64_t)1 << 26) { tok_launch_order(a, scratch, s); a.order = scratch; }
+            if (scratch && a.rows > grid && a.rows <= TOK_ORDER_ROWS && a.rows * a.V >= (int64_t)1 << 26) {
+                tok_launch_order(a, reinterpret_cast<int32_t*>(scratch), s);
+                a.order = reinterpret_cast<const int32_t*>(scratch);
+            }
         };
 #define TOK_REGS(NT, NV, FULL, PER_CU) do { if (nfull <= NT * NV) { const int grid = (int)(a.rows < 256 * PER_CU ? a.rows : 256 * PER_CU); \
         a.peel = nfull - HEAD >= NT * FULL ? 127u : 0u; in_order(grid); \
@@ -611,12 +740,12 @@ int tok_launch4(TokArgs& a, int32_t* scratch, hipStream_t s) {
     }
 }
 template <class T, int MODE>
-int tok_launch2(TokArgs& a, bool en, int32_t* scratch, hipStream_t s) {
+int tok_launch2(TokArgs& a, bool en, void* scratch, hipStream_t s) {
     if (a.avail) return en ? tok_launch4<T, MODE, true, true>(a, scratch, s) : tok_launch4<T, MODE, true, false>(a, scratch, s);
     return en ? tok_launch4<T, MODE, false, true>(a, scratch, s) : tok_launch4<T, MODE, false, false>(a, scratch, s);
 }
 template <class T>
-int tok_launch_type(TokArgs& a, int mode, bool en, int32_t* scratch, hipStream_t s) {
+int tok_launch_type(TokArgs& a, int mode, bool en, void* scratch, hipStream_t s) {
     if (mode == TOK_LOGP) return tok_launch2<T, TOK_LOGP>(a, en, scratch, s);
     if (mode == TOK_BWD) return tok_launch2<T, TOK_BWD>(a, en, scratch, s);
     return tok_launch2<T, TOK_POLICY>(a, en, scratch, s);
