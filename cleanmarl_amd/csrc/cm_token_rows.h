@@ -378,7 +378,7 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
 // Short rows: G lanes of a wave hold one row in registers (NV pieces of 16 bytes to a lane), 64 / G rows to a wave.  The row is read once,
 // its exponentials are made once and scaled into the gradient.
 template <class T, int MODE, bool AV, bool EN, int G, int NV>
-__global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
+__global__ __launch_bounds__(256, 8) void k_tok_short(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, PER = 256 / G;
     constexpr bool ENT = EN || MODE == TOK_POLICY;
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
         bool live = tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f);
         float f[NV][W];
         float x = 0.0f;
-        if (live) {
+        {  // of a row that is left out, too: waiting for its token first would cost more than the row
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int j = (k * G + gl) * W;
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(256) void k_tok_short(const TokArgs a) {
                     for (int i = 0; i < W; ++i) f[k][i] = -INFINITY;
                 }
             }
-            if (MODE != TOK_BWD) x = tok_logit<T, AV>(row, av, tok, a.V);
+            if (MODE != TOK_BWD) x = tok_logit<T, AV>(row, av, tok < 0 ? 0 : tok, a.V);
         }
         TokGrad g = {};
         if (MODE == TOK_BWD) {
