@@ -489,7 +489,8 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     constexpr int W = T::W, NW = NT / 64;
     __shared__ TokRun sh[2][NW];
     __shared__ TokSum careful[NW];
-    double st[TOK_STATS] = {};
+    __shared__ double st[TOK_STATS];  // the first thread's: in registers they would be sixteen of every thread's
+    if (threadIdx.x == 0) for (int i = 0; i < TOK_STATS; ++i) st[i] = 0.0;
     int turn = 0;
     const int tid = threadIdx.x;
     struct Row { int64_t tok; TokPolicyRow q; bool live; };
@@ -522,7 +523,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         const int slot = min(tid, nfull - 1 - k * NT);
         return tok_avail<W>(reinterpret_cast<const uint8_t*>(base(av, k * NT * W) + slot * W), 0);
     };
-    constexpr int R = NV < 8 ? NV : 8;
+    constexpr int R = NT == 1024 ? 4 : (NV < 8 ? NV : 8);
     __shared__ TokAvail<W> ok[AV ? NV : 1][AV ? NT : 1];
     tok_u4 raw[NV];
     TokAvail<W> ring[AV ? R : 1];
