@@ -27,8 +27,10 @@ struct AwArgs {
     float omb1, beta1, omb2, beta2, eps, wdf, step_size, inv_bc2, grad_scale;
     double lr, b1, b2;          // step_dev: the factors that depend on the step are made on the device
     const int32_t* step_dev;
-    const float* coef;          // clip coefficient of this step; NULL: no clipping
+    const float* coef;          // clip coefficient of this step; NULL: no clipping, or
+    const double* parts; int nparts; float max_norm; float* norm;  // the few partial sums that it is made of (nparts > 0)
 };
+constexpr int AW_FEW = 256;     // partial sums that every wave adds up by itself: a launch less for short lists
 
 typedef float aw_f4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned aw_u4 __attribute__((ext_vector_type(4), aligned(2)));
@@ -37,6 +39,11 @@ typedef _Float16 aw_h2 __attribute__((ext_vector_type(2)));
 typedef __bf16 aw_b2 __attribute__((ext_vector_type(2)));
 typedef float aw_f2 __attribute__((ext_vector_type(2)));
 
+__device__ __forceinline__ float aw_coef(float norm, float max_norm) {
+#pragma clang fp contract(off)
+    const float c = max_norm / (norm + 1e-6f);
+    return c < 1.0f || c != c ? c : 1.0f;  // a norm that is NaN reaches the parameters
+}
 __device__ __forceinline__ float aw_get(const void* p, int64_t i, int dt) {
     if (dt == CM_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];
     if (dt == CM_DTYPE_F16) return (float)reinterpret_cast<const _Float16*>(p)[i];
@@ -117,7 +124,14 @@ __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a
         step_size = (float)(a.lr / (1.0 - pow(a.b1, s)));
         inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(a.b2, s)));
     }
-    const float coef = a.coef ? a.coef[0] : 1.0f;
+    float coef = a.coef ? a.coef[0] : 1.0f;
+    if (a.nparts) {
+        double s = 0.0;
+        for (int q = threadIdx.x & 63; q < a.nparts; q += 64) s += a.parts[q];
+        const float norm = (float)sqrt(cm_wave_sum_d(s));
+        coef = aw_coef(norm, a.max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) { a.norm[0] = norm; a.norm[1] = coef; }
+    }
     const int half = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t blocks = (e.n + AW_BLOCK - 1) / AW_BLOCK, b0 = (int64_t)(blockIdx.x - e.first) * AW_CHUNK;
     const int64_t b1 = min(b0 + AW_CHUNK, blocks);
@@ -218,9 +232,9 @@ __global__ __launch_bounds__(1024) void k_adamw_coef(const double* __restrict__ 
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int w = 1; w < 16; ++w) s += sh[w];
-    const float x = (float)sqrt(s), c = max_norm / (x + 1e-6f);
+    const float x = (float)sqrt(s);
     norm[0] = x;
-    norm[1] = c < 1.0f || c != c ? c : 1.0f;  // a norm that is NaN reaches the parameters
+    norm[1] = aw_coef(x, max_norm);
 }
 
 inline size_t aw_elem(int dtype) { return dtype == CM_DTYPE_F32 ? 4 : 2; }
@@ -295,7 +309,9 @@ extern "C" int cm_adamw_multi_step(const cm_adamw_tensor_t* tensors, int n_tenso
             }
             CM_CHECK_LAUNCH("cm_adamw_multi_step");
         }
-        if (round == 0) {
+        if (round == 0 && parts > 0 && parts <= AW_FEW) {
+            a.parts = (const double*)o->ws; a.nparts = parts; a.max_norm = (float)o->max_norm; a.norm = o->out_norm;
+        } else if (round == 0) {
             hipLaunchKernelGGL(k_adamw_coef, dim3(1), dim3(1024), 0, s, (const double*)o->ws, parts, (float)o->max_norm, o->out_norm);
             CM_CHECK_LAUNCH("cm_adamw_multi_step/norm");
             a.coef = o->out_norm + 1;
