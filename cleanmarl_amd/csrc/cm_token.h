@@ -163,7 +163,10 @@ __device__ __forceinline__ void tok_store(typename T::elem* row, int j, int V, c
 struct TokSum { float m, s, u; };
 
 constexpr float TOK_LN2 = 0.6931471805599453f, TOK_FAR = -1e20f;  // products with e^t = 0 stay 0 where t2 is clamped to TOK_FAR
-struct TokScale { float nat, bin; };  // 1 / T and log2(e) / T
+// 1 / T, and log2(e) / T in 64 bits and as the sum of two floats: rounded to one, it would move every logit of a row the same way, and what moves
+// each log-probability by 1e-7 moves the sum over a long answer by 1e-4
+// (lo > 0, so that its product with -inf is -inf)
+struct TokScale { float nat, bin, lo; double full; };
 
 __device__ __forceinline__ float tok_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -184,14 +187,14 @@ __device__ __forceinline__ void tok_merge(TokSum& a, TokSum b, float bin) {
     if constexpr (EN) a.u += b.u;
 }
 template <bool EN, int W>
-__device__ __forceinline__ void tok_add(TokSum& a, const float (&f)[W], float bin) {
+__device__ __forceinline__ void tok_add(TokSum& a, const float (&f)[W], float bin, float lo) {
     float m = a.m;
 #pragma unroll
     for (int i = 0; i < W; ++i) m = fmaxf(m, f[i]);
     tok_raise<EN>(a, m, bin);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float d = (f[i] - m) * bin, e = tok_exp2(d);
+        const float x = f[i] - m, d = fmaf(x, lo, x * bin), e = tok_exp2(d);
         a.s += e;
         if constexpr (EN) a.u = fmaf(e, fmaxf(d, TOK_FAR), a.u);
     }
@@ -236,7 +239,7 @@ __device__ __forceinline__ void run_raise(TokRun& a, float M) {
 }
 // CLAMP: -inf among the logits is ordinary (unavailable columns), its product with e^t = 0 must not be NaN
 template <bool EN, bool CLAMP, int W>
-__device__ __forceinline__ void run_add(TokRun& a, const float (&f)[W], float c) {
+__device__ __forceinline__ void run_add(TokRun& a, const float (&f)[W], float c, float lo) {
     float m = f[0];
 #pragma unroll
     for (int i = 1; i < W; ++i) m = fmaxf(m, f[i]);
@@ -244,7 +247,9 @@ __device__ __forceinline__ void run_add(TokRun& a, const float (&f)[W], float c)
     if (m > a.M + TOK_SLACK) run_raise<EN>(a, m);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        const float t = fmaf(f[i], c, -a.M), e = tok_exp2(t);
+        float t = fmaf(f[i], c, -a.M);
+        t = fmaf(f[i], lo, t);
+        const float e = tok_exp2(t);
         a.s += e;
         if constexpr (EN) a.u = fmaf(e, CLAMP ? fmaxf(t, TOK_FAR) : t, a.u);
     }
@@ -282,6 +287,13 @@ template <bool EN>
 __device__ __forceinline__ bool run_ordinary(const TokRun& a) {
     return a.s > 0.0f && a.s < INFINITY && fabsf(a.M) <= TOK_LARGE && (!EN || fabsf(a.u) < INFINITY);
 }
+
+// The gradients do without `lo`: 2^(x c - M) / s' with the s' that makes the two agree near the maximum, where x is M / c
+__device__ __forceinline__ float run_sum(const TokRun& z, const TokScale& c) { return z.s * tok_exp2(-z.M * (c.lo / c.bin)); }
+
+// log-probability of a logit x from the row's sums: t in 64 bits (one rounding at the end), log s in 32, or in 64 for sums of many of them
+__device__ __forceinline__ float run_logp(float x, float M, float logs, const TokScale& c) { return (float)(((double)x * c.full - (double)M) * 0.6931471805599453 - (double)logs); }
+__device__ __forceinline__ float tok_logp(float x, float m, float logs, const TokScale& c) { return (float)(((double)x - (double)m) * c.full * 0.6931471805599453 - (double)logs); }
 
 // ---------------------------------------------------------------- what a row's backward needs
 // dx_j = a [j = token] - b p_j + h p_j (log p_j + H), all already divided by T; p_j = e^t rs, log p_j + H = t + K
@@ -355,7 +367,7 @@ constexpr int TOK_STATS = CM_NUM_STATS, TOK_MAX_GRID = 2048;
 struct TokArgs {
     const void* logits; int64_t ld; const uint8_t* avail; int64_t avail_ld; const void* token; int token_bytes;
     int64_t rows; int V; TokScale c;
-    float *logp, *entropy; float2* keep;                                     // forward: keep = (m, s), (M, -s) in the form of TokRun, s = 0 for a row that is left out
+    float *logp, *entropy; double* logp64; float2* keep;                                     // forward: keep = (m, s), (M, -s) in the form of TokRun, s = 0 for a row that is left out
     const float2* keep_in; const float *entropy_in, *d_logp, *d_entropy;     // backward
     void* dlogits; int64_t dld;
     const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy

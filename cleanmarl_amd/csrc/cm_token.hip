@@ -97,7 +97,7 @@ __global__ __launch_bounds__(1024) void k_tok_order(const void* __restrict__ tok
 // One workgroup per pair: log-probabilities of its two sequences (64-bit sums: thousands of terms, and only their difference counts),
 // the margin, the loss and the factor that every row of the two sequences gets.
 struct PrefArgs {
-    const float* logp; const int32_t* seq_start; int pairs; int64_t rows; const float* ref;
+    const double* logp; const int32_t* seq_start; int pairs; int64_t rows; const float* ref;
     double beta, smooth, scale; int kind;
     float *coef, *margin, *seq_logp; double* part;  // coef: one factor per row
 };
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256) void k_pref_pair(const PrefArgs a) {
         const int q = i + k * a.pairs;
         b[k] = max((int64_t)a.seq_start[q], (int64_t)0); e[k] = min((int64_t)a.seq_start[q + 1], a.rows);
         double s = 0.0;
-        for (int64_t r = b[k] + threadIdx.x; r < e[k]; r += 256) s += (double)a.logp[r];
+        for (int64_t r = b[k] + threadIdx.x; r < e[k]; r += 256) s += a.logp[r];
         s = cm_wave_sum_d(s);
         if ((threadIdx.x & 63) == 0) sh[k][threadIdx.x >> 6] = s;
     }
@@ -188,7 +188,10 @@ TokArgs tok_args(const cm_token_rows_t* t) {
     TokArgs a = {};
     a.logits = t->logits; a.ld = t->ld; a.avail = t->avail; a.avail_ld = t->avail_ld; a.token = t->token; a.token_bytes = t->token_bytes;
     a.rows = t->rows; a.V = t->vocab;
-    a.c.nat = (float)(1.0 / t->temperature); a.c.bin = (float)(1.4426950408889634074 / t->temperature);
+    a.c.full = 1.4426950408889634074 / t->temperature;
+    a.c.nat = (float)(1.0 / t->temperature); a.c.bin = (float)a.c.full;
+    if ((double)a.c.bin > a.c.full) a.c.bin = nextafterf(a.c.bin, 0.0f);
+    a.c.lo = fmaxf((float)(a.c.full - (double)a.c.bin), FLT_MIN);
     return a;
 }
 
@@ -255,7 +258,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
 
 extern "C" size_t cm_preference_workspace_bytes(int64_t rows, int vocab, int pairs) {
     if (rows < 0 || vocab < 1 || pairs < 1) return 0;
-    return tok_up((size_t)rows * sizeof(float2)) + 2 * tok_up((size_t)rows * sizeof(float)) +
+    return tok_up((size_t)rows * sizeof(float2)) + tok_up((size_t)rows * sizeof(double)) + tok_up((size_t)rows * sizeof(float)) +
            tok_up((size_t)pairs * TOK_STATS * sizeof(double)) + tok_scratch(rows);
 }
 
@@ -275,12 +278,12 @@ extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* se
     CM_REQUIRE(ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "cm_preference_fwd_bwd: workspace too small (%zu < %zu) or not 16-byte aligned", ws_bytes, need);
     char* w = (char*)ws;
     float2* keep = (float2*)w; w += tok_up((size_t)t->rows * sizeof(float2));
-    float* logp = (float*)w; w += tok_up((size_t)t->rows * sizeof(float));
+    double* logp = (double*)w; w += tok_up((size_t)t->rows * sizeof(double));
     float* coef = (float*)w; w += tok_up((size_t)t->rows * sizeof(float));
     double* part = (double*)w; w += tok_up((size_t)pairs * TOK_STATS * sizeof(double));
     hipStream_t s = (hipStream_t)stream;
     TokArgs a = tok_args(t);
-    a.range_lo = seq_start; a.range_hi = seq_start + 2 * pairs; a.logp = logp; a.keep = keep;
+    a.range_lo = seq_start; a.range_hi = seq_start + 2 * pairs; a.logp64 = logp; a.keep = keep;
     tok_launch(a, t->dtype, TOK_LOGP, false, w, s);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/logp");
     PrefArgs p = {logp, seq_start, pairs, t->rows, logp_ref, beta, label_smoothing, scale, kind, coef, margin, seq_logp, part};

@@ -20,6 +20,10 @@ __device__ __forceinline__ float tok_logit(const typename T::elem* row, const ui
     return !AV || av[tok] ? T::get(row[tok]) : -INFINITY;
 }
 
+// the same in 64 bits, for sums over many rows; s = 0: a row that is left out
+__device__ __forceinline__ double run_logp64(float x, float M, float s, const TokScale& c) { return ((double)x * c.full - (double)M) * 0.6931471805599453 - log((double)s); }
+__device__ __forceinline__ double tok_logp64(float x, float m, float s, const TokScale& c) { return s == 0.0f ? 0.0 : ((double)x - (double)m) * c.full * 0.6931471805599453 - log((double)s); }
+
 // scalars of the clipped policy loss of one row: adds its statistics to st (where `add`), returns g = dloss / dlogp and h = the entropy's factor
 struct TokPolicyRow { float old, adv, ref, w; };
 __device__ __forceinline__ TokPolicyRow tok_policy_load(const TokArgs& a, int64_t r) {
@@ -59,7 +63,7 @@ __device__ __forceinline__ TokSum tok_careful_sum(const typename T::elem* row, c
     for (int j = threadIdx.x * T::W; j < a.V; j += NT * T::W) {
         float f[T::W];
         tok_load<T, AV>(row, av, j, a.V, f);
-        tok_add<EN>(z, f, a.c.bin);
+        tok_add<EN>(z, f, a.c.bin, a.c.lo);
     }
     tok_block<EN, NT / 64>(z, a.c.bin, sh);
     return z;
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
             if (live) {
                 const float logs = logf(z.s);
                 g.m = z.m; g.rs = 1.0f / z.s;
-                logp = (x - z.m) * a.c.nat - logs;
+                logp = tok_logp(x, z.m, logs, a.c);
                 g.K = -z.u * g.rs * TOK_LN2;
                 float gg, hh;
                 tok_policy_row(a, q, logp, logs + g.K, threadIdx.x == 0, st, gg, hh);
@@ -165,28 +169,31 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
 #pragma unroll
                         for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
                     }
-                    run_add<EN, true>(z, f, a.c.bin);
+                    run_add<EN, true>(z, f, a.c.bin, a.c.lo);
                 }
             }
             const int je = shape.edge(tid, W);
-            if (tid < shape.edges && (!AV || av[je])) { const float one[1] = {T::get(row[je])}; run_add<EN, true>(z, one, a.c.bin); }
+            if (tid < shape.edges && (!AV || av[je])) { const float one[1] = {T::get(row[je])}; run_add<EN, true>(z, one, a.c.bin, a.c.lo); }
             run_block<EN, NW>(z, sh[turn]);
             turn ^= 1;
             if (run_ordinary<EN>(z)) {
                 const float logs = logf(z.s);
-                logp = fmaf(x, a.c.bin, -z.M) * TOK_LN2 - logs;
+                logp = run_logp(x, z.M, logs, a.c);
                 H = logs - z.u / z.s * TOK_LN2;
-                keep = make_float2(z.M, -z.s);
+                keep = make_float2(z.M, -run_sum(z, a.c));
+                if (a.logp64 && tid == 0) a.logp64[r] = run_logp64(x, z.M, z.s, a.c);
             } else {
                 const TokSum y = tok_careful_sum<T, AV, EN, NT>(row, av, a, careful);
                 const float logs = logf(y.s);
-                if (y.s != 0.0f) { logp = (x - y.m) * a.c.nat - logs; H = logs - y.u / y.s * TOK_LN2; }
+                if (y.s != 0.0f) { logp = tok_logp(x, y.m, logs, a.c); H = logs - y.u / y.s * TOK_LN2; }
                 keep = make_float2(y.m, y.s);
+                if (a.logp64 && tid == 0) a.logp64[r] = tok_logp64(x, y.m, y.s, a.c);
                 __syncthreads();  // `careful` is free again
             }
         }
         if (tid == 0) {
             if (a.logp) a.logp[r] = logp;
+            if (a.logp64 && tok < 0) a.logp64[r] = 0.0;
             if (EN && a.entropy) a.entropy[r] = H;
             if (a.keep) a.keep[r] = keep;
         }
@@ -215,10 +222,10 @@ __global__ __launch_bounds__(NT) void k_tok_part(const TokArgs a) {
         if (AV) tok_mask_raw<T>(tok_avail<W>(av + shape.head, i * W), raw);
         float f[W];
         T::unpack(raw, f);
-        run_add<EN, true>(z, f, a.c.bin);
+        run_add<EN, true>(z, f, a.c.bin, a.c.lo);
     }
     const int je = shape.edge(tid, W);
-    if (seg == 0 && tid < shape.edges && (!AV || av[je])) { const float one[1] = {T::get(row[je])}; run_add<EN, true>(z, one, a.c.bin); }
+    if (seg == 0 && tid < shape.edges && (!AV || av[je])) { const float one[1] = {T::get(row[je])}; run_add<EN, true>(z, one, a.c.bin, a.c.lo); }
     run_block<EN, NW>(z, sh);
     if (tid == 0) a.split[r * a.segs + seg] = make_float4(z.M, z.s, z.u, seg == 0 ? tok_logit<T, AV>(row, av, tok, a.V) : 0.0f);
 }
@@ -260,18 +267,21 @@ __global__ __launch_bounds__(NT) void k_tok_join(const TokArgs a) {
         }
         if (here && lane == 0) {
             float logp = 0.0f, H = 0.0f, g = 0.0f, h = 0.0f;
+            double logp64 = 0.0;
             float2 keep = {0.0f, 0.0f};
             if (counts) {
                 const TokSum y = ordinary ? TokSum{0.0f, z.s, z.u} : sums[slot];
                 const float logs = logf(y.s);
                 if (y.s != 0.0f) {
-                    logp = (ordinary ? fmaf(x, a.c.bin, -z.M) * TOK_LN2 : (x - y.m) * a.c.nat) - logs;
+                    logp = ordinary ? run_logp(x, z.M, logs, a.c) : tok_logp(x, y.m, logs, a.c);
                     if (ENT) H = logs - y.u / y.s * TOK_LN2;
                     if (MODE == TOK_POLICY) tok_policy_row(a, q, logp, H, true, st, g, h);
                 }
-                keep = ordinary ? make_float2(z.M, -z.s) : make_float2(y.m, y.s);
+                keep = ordinary ? make_float2(z.M, -run_sum(z, a.c)) : make_float2(y.m, y.s);
+                logp64 = ordinary ? run_logp64(x, z.M, z.s, a.c) : tok_logp64(x, y.m, y.s, a.c);
             }
             if (a.logp) a.logp[r] = logp;
+            if (a.logp64) a.logp64[r] = logp64;
             if (a.keep) a.keep[r] = keep;
             if (ENT && a.entropy) a.entropy[r] = H;
             if (MODE == TOK_POLICY) { a.g_out[r] = g; a.h_out[r] = -h; }
@@ -427,7 +437,7 @@ __global__ __launch_bounds__(256, 8) void k_tok_short(const TokArgs a) {
                 for (int k = 0; k < NV; ++k)
 #pragma unroll
                     for (int i = 0; i < W; ++i) {
-                        const float t = (f[k][i] - m) * a.c.bin, e = tok_exp2(t);
+                        const float d = f[k][i] - m, t = fmaf(d, a.c.lo, d * a.c.bin), e = tok_exp2(t);
                         s += e;
                         if (ENT) u = fmaf(e, fmaxf(t, TOK_FAR), u);
                     }
@@ -439,7 +449,7 @@ __global__ __launch_bounds__(256, 8) void k_tok_short(const TokArgs a) {
             if (live) {
                 const float logs = logf(s);
                 g.m = m; g.rs = 1.0f / s;
-                logp = (x - m) * a.c.nat - logs;
+                logp = tok_logp(x, m, logs, a.c);
                 if (ENT) { g.K = -u * g.rs * TOK_LN2; H = logs + g.K; }
             }
             if (MODE == TOK_POLICY && live) {
@@ -449,6 +459,7 @@ __global__ __launch_bounds__(256, 8) void k_tok_short(const TokArgs a) {
             }
             if (gl == 0) {
                 if (a.logp) a.logp[r] = logp;
+                if (MODE == TOK_LOGP && a.logp64) a.logp64[r] = tok_logp64(x, m, live ? s : 0.0f, a.c);
                 if (EN && a.entropy) a.entropy[r] = H;
                 if (a.keep) a.keep[r] = make_float2(m, live ? s : 0.0f);
             }
@@ -572,7 +583,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         if (now.live) {
             lastf = edge && last_ok ? T::get(last) : -INFINITY;
             const float one[1] = {lastf};
-            run_add<true, true>(z, one, a.c.bin);
+            run_add<true, true>(z, one, a.c.bin, a.c.lo);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 if (k >= FULL && k * NT >= nfull) break;
@@ -580,12 +591,12 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
                 float f[W];
                 T::unpack(raw[k], f);
                 if (k < FULL) {
-                    run_add<true, AV>(z, f, a.c.bin);
+                    run_add<true, AV>(z, f, a.c.bin, a.c.lo);
                 } else {
                     const bool here = tid + k * NT < nfull;
 #pragma unroll
                     for (int i = 0; i < W; ++i) f[i] = here ? f[i] : -INFINITY;
-                    run_add<true, true>(z, f, a.c.bin);
+                    run_add<true, true>(z, f, a.c.bin, a.c.lo);
                 }
                 asm volatile("" : "+v"(z.M), "+v"(z.s), "+v"(z.u));  // one piece after the other: interleaved, the floats of all of them would be live at once
                 __builtin_amdgcn_sched_barrier(0);
@@ -608,12 +619,12 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         if (live) {
             const float logs = logf(s);
             g.m = y.m; g.rs = 1.0f / s;
-            logp = (ordinary ? fmaf(x, a.c.bin, -z.M) * TOK_LN2 : (x - y.m) * a.c.nat) - logs;
+            logp = ordinary ? run_logp(x, z.M, logs, a.c) : tok_logp(x, y.m, logs, a.c);
             g.K = -(ordinary ? z.u : y.u) * g.rs * TOK_LN2; H = logs + g.K;
             float gg, hh;
             tok_policy_row(a, now.q, logp, H, tid == 0, st, gg, hh);
             g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
-            if (ordinary) gr = run_grad_row<T, EN>(z.M, s, g.K, g.b, g.h);
+            if (ordinary) { const float sg = run_sum(z, a.c); gr = run_grad_row<T, EN>(z.M, sg, H - logf(sg), g.b, g.h); }
         }
         if (tid == 0 && a.logp) a.logp[r] = logp;
         {
