@@ -331,7 +331,7 @@ __device__ __forceinline__ RunGrad run_grad_row(float M, float s, float K, float
     g.fold = !HE && T::W == 8 && fabsf(M) <= 128.0f && !(fabsf(g.shift) > 256.0f && b != 0.0f);
     return g;
 }
-template <class T, bool HE, bool CLAMP>
+template <class T, bool HE>
 __device__ __forceinline__ tok_u4 run_grad(const tok_u4& raw, const RunGrad& g, float c) {
     float f[T::W], d[T::W];
     T::unpack(raw, f);
@@ -347,8 +347,7 @@ __device__ __forceinline__ tok_u4 run_grad(const tok_u4& raw, const RunGrad& g, 
     for (int i = 0; i < T::W; ++i) {
         const float t = fmaf(f[i], c, -g.M), e = tok_exp2(t);
         if constexpr (HE) {
-            const float l = fmaf(t, TOK_LN2, g.K);
-            d[i] = e * fmaf(g.hrs, CLAMP ? fmaxf(l, TOK_FAR) : l, g.brs);
+            d[i] = e * fmaf(g.hrs, fmaxf(fmaf(t, TOK_LN2, g.K), TOK_FAR), g.brs);  // e = 0 where it is clamped
         } else d[i] = e * g.brs;
     }
     return T::pack(d);

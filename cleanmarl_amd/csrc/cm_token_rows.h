@@ -355,7 +355,7 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
             if (AV) tok_mask_raw<T>(ok[k], raw[k]);
             tok_u4 d;
             if (run) {
-                d = run_grad<T, EN, true>(raw[k], gr, a.c.bin);
+                d = run_grad<T, EN>(raw[k], gr, a.c.bin);
             } else {
                 float f[W], v[W];
                 T::unpack(raw[k], f);
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
                 for (int k = 0; k < NV; ++k) {
                     asm volatile("" : "+v"(raw[k]));  // unpacked again: the floats of the first sweep would be kept, at two registers for one
                     if (k < FULL || tid + k * NT < nfull) {
-                        __builtin_nontemporal_store((typename T::vec)run_grad<T, EN, AV>(raw[k], gr, a.c.bin), at(dbody, k));
+                        __builtin_nontemporal_store((typename T::vec)run_grad<T, EN>(raw[k], gr, a.c.bin), at(dbody, k));
                     }
                     if (AV) {
                         ok[k][tid] = ring[k % R];

@@ -229,6 +229,31 @@ def test_long_lists_missing_gradients_and_empty_tensors(bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_of_more_than_31_bits(bits):
+    """Elements behind the 2^31st: the last ones and some in the middle are held to the rule; the norm counts them all."""
+    from cleanmarl_amd.adamw import MultiAdamW
+    n = (1 << 31) + 777
+    p = torch.full((n,), 0.5, dtype=torch.bfloat16, device="cuda")
+    g = torch.full((n,), 2.0 ** -10, dtype=torch.bfloat16, device="cuda")
+    spots = [slice(0, 512), slice((1 << 30) - 256, (1 << 30) + 256), slice(n - 777, n)]
+    for i, sl in enumerate(spots):
+        g[sl] = tensors([sl.stop - sl.start], [torch.bfloat16], i, scale=0.01)[0]
+    other = torch.zeros(5, device="cuda")
+    opt = MultiAdamW([p, other], state_bits=bits, max_norm=1.0, **H)
+    opt.step([g, torch.ones(5, device="cuda")])
+    total = float(sum(c.float().double().square().sum() for c in g.split(1 << 28))) + 5
+    assert abs(opt.norm[0].item() - math.sqrt(total)) <= 2 * U * math.sqrt(total)
+    coef = opt.norm[1].item()
+    for sl in spots:
+        k = sl.stop - sl.start
+        want, m, v = plain_step(torch.full((k,), 0.5, dtype=torch.bfloat16, device="cuda"), g[sl], torch.zeros(k, device="cuda"), torch.zeros(k, device="cuda"), 1, coef)
+        assert torch.equal(p[sl], want.to(torch.bfloat16))
+    want, _, _ = plain_step(torch.zeros(5, device="cuda"), torch.ones(5, device="cuda"), torch.zeros(5, device="cuda"), torch.zeros(5, device="cuda"), 1, coef)
+    assert torch.equal(other, want)
+
+
+@pytest.mark.gpu
 def test_states_of_zero_tiny_and_huge_gradients():
     from cleanmarl_amd.adamw import MultiAdamW
     n = 1024

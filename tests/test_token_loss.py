@@ -4,6 +4,8 @@ Tolerances are counted from roundings (U = 2^-24, half a step of fp32 at 1):
   * t = (x - m) / T carries <= 3 U relative (difference, reciprocal temperature, product); with v_exp_f32 good to 2 U and sum p |t| <= log V, a
     thread's sum of n terms and the <= 24 merges behind it put  U (3 log V + 4 + n + 24)  on s;
   * log p_token = t - log s: that, plus 3 U |t| + 2 U log s + U |log p|;  H = log s - u / s: u's terms carry the same again times their |t|;
+  * p_j = e^t / s of a gradient does without the low part of log2(e) / T (up to 2 U of it): 2 U more on |t|, and 2 U * 16 where the reference
+    point of the sums lags its largest 16 (in powers of two) behind the row's maximum;
   * a gradient entry: the relative errors of its factors, then one rounding to the logits' type, finfo.eps / 2 of the value.
 n is counted as V / 64 + 16: no kernel gives one thread more than that.
 """
@@ -54,7 +56,7 @@ class Bars:
         tt = torch.where(tt == -math.inf, 0.0, tt)
         self.logp = torch.where(live, self.s + 3 * U * tt.abs() + 2 * U * logs[:, 0] + U * lp.gather(1, at)[:, 0].abs(), 0.0)
         self.H = torch.where(live, 2 * self.s * (1 + logs[:, 0]) + 4 * U * (H + logs[:, 0]) + 4 * U, 0.0)
-        self.p = self.s + 3 * U * torch.where(p > 0, t.abs(), 0.0) + 4 * U  # relative error of p_j
+        self.p = self.s + 5 * U * torch.where(p > 0, t.abs(), 0.0) + (4 + 32) * U  # relative error of p_j
 
 
 def rounded(want, dtype):
@@ -81,8 +83,9 @@ def grad_bar(ref, bars, token, g, h, g_rel, T, want, dtype):
     lpz = torch.where(p > 0, lp, 0.0)
     a = g.abs()[:, None] * (one + p) * (bars.p + g_rel[:, None] + 6 * U)
     b = h.abs()[:, None] * p * ((lpz.abs() + H[:, None]) * (bars.p + 8 * U) + bars.H[:, None] + bars.s + 3 * U * (lpz.abs() + logs))
-    bar = (a + b) / T
-    return bar + rounded(want.abs() + bar, dtype) + 1e-37
+    flushed = 2.0 ** -126 * (1 + g.abs()[:, None] + h.abs()[:, None] * (lpz.abs() + H[:, None]))  # v_exp_f32 gives 0 for what is below 2^-126
+    bar = (a + b + flushed) / T
+    return bar + rounded(want.abs() + bar, dtype)
 
 
 def close(got, want, bar, what):
@@ -355,6 +358,118 @@ def test_policy_loss(rows, V, dtype):
         check_stats(over.stats)
 
 
+def _policy_case(x, tok, mask, T, seed, kl=0.1, ent=0.02):
+    """Everything of a policy call on given logits but the comparison of its statistics: (result, log-probabilities, gradient, its bar)."""
+    from cleanmarl_amd import token_loss as TL
+    rows, V = x.shape
+    gen = torch.Generator().manual_seed(seed)
+    ref = reference(x, tok, mask, T)
+    bars = Bars(ref, V, tok)
+    live = ref[5]
+    taken = torch.where(live, ref[2].gather(1, tok.cpu().clamp(min=0).long()[:, None])[:, 0], 0.0)
+    old = (taken - torch.randn(rows, generator=gen).double().clamp(-2, 2) * 0.05).float()
+    adv, refp = torch.randn(rows, generator=gen), (taken + 0.3).float()
+    want = policy_reference(ref, tok, old.double(), adv.double(), refp.double(), torch.ones(rows).double(), 0.2, 0.2, kl, ent)
+    dwant = torch.where(live[:, None], grad_reference(ref, tok, want["g"], want["h"], T), 0.0)
+    delta = bars.logp + U * (taken.abs() + 4)
+    g_abs = (adv.double() * want["rho"]).abs() * (delta + 6 * U) + (torch.exp(refp.double() - taken) + 1) * kl * (delta + 6 * U)
+    g_rel = torch.where(want["g"] != 0, g_abs / want["g"].abs().clamp(min=1e-300), 0.0)
+    bar = grad_bar(ref, bars, tok, want["g"], want["h"], g_rel, T, dwant, x.dtype)
+    call = lambda out=None: TL.policy_loss_fwd_bwd(x, tok, old.cuda(), adv.cuda(), logp_ref=refp.cuda(), avail=mask, temperature=T, kl_coef=kl, entropy_coef=ent, out=out)  # noqa: E731
+    return call, want["logp"], bars.logp + U * want["logp"].abs(), dwant, bar, live
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [3, 40, 700, 5000, 70000, 140002])
+def test_policy_loss_on_rows_of_every_size(V, dtype):
+    """Rows beside each other that are ordinary, far from zero, of one value (the type's lowest), with -inf among them, or all -inf; small temperatures."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(9, V, generator=gen) * 2
+    x[1] = x[1] * 0.5 + (30000 if dtype == torch.float16 else 1e5)
+    x[2] = LOWEST[dtype]
+    x[3, 1::2] = -math.inf
+    x[4] = -math.inf
+    x[5] = LOWEST[dtype]
+    x[5, 0] = 1.0
+    x[6] = x[6] - (30000 if dtype == torch.float16 else 3e4)
+    x[7, :] = 0.25
+    x = x.to(dtype)
+    tok = torch.tensor([0, V - 1, 0, 0, 0, 0, V // 2, V // 2, V - 1])
+    tok[6] = int(x[6].float().argmax())
+    tok[1] = int(x[1].float().argmax())
+    for T in (1.0, 0.01):
+        xs, toks = x.cuda(), tok.cuda()
+        call, lp, lp_bar, dwant, bar, live = _policy_case(xs, toks, None, T, V, kl=0.0)
+        r = call()
+        close(r.logp, lp, lp_bar, "logp")
+        close(r.dlogits, dwant, bar, "dlogits")
+        assert int(r.stats[5]) == int(live.sum()) == 8
+        over = call(out=xs)
+        close(over.dlogits, dwant, bar, "dlogits in place")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V, dtype", [(65536, torch.bfloat16), (32768, torch.float32), (65601, torch.float16)])
+def test_rows_that_count_come_first(V, dtype):
+    """Long batches are taken in the order of the rows that count.  The same rows in slices, each too short for an order, give the same values: bit by bit where
+    every row starts at the same alignment, else within the bars of both (twice one bar)."""
+    from cleanmarl_amd import token_loss as TL
+    rows = 2300 if V % 64 == 0 else 1100
+    gen = torch.Generator("cuda").manual_seed(V)
+    x = torch.randn(rows, V, generator=gen, device="cuda", dtype=dtype)
+    tok = torch.randint(V, (rows,), generator=gen, device="cuda")
+    tok[torch.rand(rows, generator=gen, device="cuda") < 0.3] = -1
+    w = (torch.rand(rows, generator=gen, device="cuda") < 0.8).float()
+    mask = (torch.rand(rows, V, generator=gen, device="cuda", dtype=torch.float16) < 0.7).to(torch.uint8) if V % 2 else None
+    old, adv = torch.randn(rows, generator=gen, device="cuda") - 12, torch.randn(rows, generator=gen, device="cuda")
+    r = TL.policy_loss_fwd_bwd(x, tok, old, adv, weight=w, avail=mask, entropy_coef=0.01)
+    total = torch.zeros(8, dtype=torch.float64)
+    for a in range(0, rows, 230):
+        b = min(rows, a + 230)
+        part = TL.policy_loss_fwd_bwd(x[a:b], tok[a:b], old[a:b], adv[a:b], weight=w[a:b], avail=None if mask is None else mask[a:b], entropy_coef=0.01,
+                                      out=torch.empty(b - a + 1, V, dtype=dtype, device="cuda")[:b - a] if V % 64 == 0 else None)
+        if V % 64 == 0:
+            assert torch.equal(part.dlogits, r.dlogits[a:b]) and torch.equal(part.logp, r.logp[a:b])
+        else:
+            # each side is within U (3 log V + V / 64 + 44 + 5 |t| + 48) of the size of its terms, p (|g| + |h| (|log p| + H)), and rounded once (together one
+            # whole step): the entropy's term and the loss's may cancel, so the result's own size is no measure
+            s_bar = U * (3 * math.log(V) + V / 64 + 92)
+            assert bool(((part.logp == r.logp[a:b]) | ((part.logp - r.logp[a:b]).abs() <= 2 * (s_bar + 40 * U))).all())  # (-inf: a token that is not available)
+            z = x[a:b].double().masked_fill(mask[a:b] == 0, -1e5)
+            lp = torch.log_softmax(z, 1)
+            size = lp.exp() * ((adv[a:b].double() * torch.exp(r.logp[a:b].double() - old[a:b].double())).abs()[:, None] + 0.01 * (lp.abs() + math.log(V)))
+            bar = 2 * size * (s_bar + 5 * U * lp.abs().clamp(max=1000)) + torch.finfo(dtype).eps * r.dlogits[a:b].double().abs() * 1.01 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+            assert bool(((part.dlogits.double() - r.dlogits[a:b].double()).abs() <= bar).all())
+        total += part.stats.double().cpu()
+    dead = (tok < 0) | (w == 0)
+    assert bool((r.dlogits[dead] == 0).all()) and bool((r.logp[dead] == 0).all()) and int(r.stats[5]) == rows - int(dead.sum()) - 0
+    got = r.stats.double().cpu()  # (an unavailable token makes the divergence infinite on both sides)
+    assert bool(((got == total) | ((got - total).abs() <= 1e-5 * (1 + total.abs()))).all())
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Rows whose distance in elements does not fit 31 bits, and products of row and stride that do not fit 32."""
+    from cleanmarl_amd import token_loss as TL
+    for V, rows in ((1000, 3), (7, 3)):
+        ld = (1 << 31) + 8
+        store = torch.empty(ld * (rows - 1) + V, dtype=torch.float16, device="cuda")
+        x = store.as_strided((rows, V), (ld, 1))
+        small = (torch.randn(rows, V, generator=torch.Generator().manual_seed(V)) * 2).to(torch.float16).cuda()
+        x.copy_(small)
+        tok, one = torch.tensor([1, 0, V - 1]).cuda(), torch.ones(rows).cuda()
+        a, b = TL.token_logprob(x, tok, entropy=True, keep=True), TL.token_logprob(small, tok, entropy=True, keep=True)
+        assert bool(((a.logp - b.logp).abs() <= 1e-5).all()) and bool(((a.entropy - b.entropy).abs() <= 1e-5).all())
+        want = TL.policy_loss_fwd_bwd(small, tok, b.logp, one)
+        da = TL.token_logprob_bwd(x, tok, a, one)
+        db = TL.token_logprob_bwd(small, tok, b, one)
+        assert bool(((da.float() - db.float()).abs() <= db.float().abs() * 2.0 ** -10 + 2.0 ** -24).all())
+        got = TL.policy_loss_fwd_bwd(x, tok, b.logp, one, out=x)
+        assert bool(((got.dlogits.float() - want.dlogits.float()).abs() <= want.dlogits.float().abs() * 2.0 ** -10 + 2.0 ** -24).all())
+        del store, x, got
+
+
 @pytest.mark.gpu
 def test_policy_gradient_against_differences():
     """Central differences of the loss statistic, one logit at a time.  Step 2^-7: a loss good to 2^-20 gives 2^-13 / 2, the third derivative
@@ -465,36 +580,45 @@ def test_preference_loss_far_margins_and_refusals():
 # ---------------------------------------------------------------------------------------------------------------- streams, graphs
 @pytest.mark.gpu
 def test_calls_on_two_streams_and_in_graphs():
-    """Two streams at once, and two captured graphs replayed in turn with eager work between: every result is the eager one."""
+    """Two streams at once, and captured graphs replayed in turn with eager work between: every result is the eager one."""
     from cleanmarl_amd import token_loss as TL
-    probs = []
-    for seed, (rows, V) in enumerate([(40, 30001), (300, 700)]):
-        x, tok, mask, gen = problem(rows, V, torch.bfloat16, seed, False)
-        old, adv = torch.randn(rows, generator=gen).cuda() - 8, torch.randn(rows, generator=gen).cuda()
-        probs.append((x, tok, old, adv))
-    call = lambda p: TL.policy_loss_fwd_bwd(*p, clip_high=0.3)  # noqa: E731
-    want = [call(p) for p in probs]
+    gen = torch.Generator("cuda").manual_seed(5)
+    calls = []
+    for rows, V, dtype in ((40, 30001, torch.bfloat16), (300, 700, torch.bfloat16), (5, 131072, torch.float16), (1100, 65536, torch.bfloat16), (900, 6, torch.float32)):
+        x = torch.randn(rows, V, generator=gen, device="cuda", dtype=dtype)
+        tok = torch.randint(V, (rows,), generator=gen, device="cuda")
+        tok[::7] = -1
+        old, adv = torch.randn(rows, generator=gen, device="cuda") - 8, torch.randn(rows, generator=gen, device="cuda")
+        calls.append(lambda x=x, tok=tok, old=old, adv=adv: TL.policy_loss_fwd_bwd(x, tok, old, adv, clip_high=0.3, entropy_coef=0.01))
+
+        def scored(x=x, tok=tok, adv=adv):
+            f = TL.token_logprob(x, tok, entropy=True, keep=True)
+            return f.logp, f.entropy, TL.token_logprob_bwd(x, tok, f, adv, d_entropy=adv)
+        calls.append(scored)
+        seq = torch.tensor([0, rows // 4, rows // 2, rows // 2 + 1, rows], dtype=torch.int32, device="cuda")
+        calls.append(lambda x=x, tok=tok, seq=seq: TL.preference_loss_fwd_bwd(x, tok, seq, torch.zeros(4, device="cuda")))
+    want = [c() for c in calls]
     torch.cuda.synchronize()
+    same = lambda a, b: all(torch.equal(u, v) for u, v in zip(a, b))  # noqa: E731
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
-    for _ in range(3):
+    for _ in range(2):
         got = []
-        for s, p in zip(streams, probs):
-            with torch.cuda.stream(s):
-                got.append(call(p))
+        for i, c in enumerate(calls):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append(c())
         torch.cuda.synchronize()
-        for a, b in zip(got, want):
-            assert all(torch.equal(u, v) for u, v in zip(a, b))
+        assert [same(a, b) for a, b in zip(got, want)] == [True] * len(calls)
     graphs, outs = [], []
-    for p in probs:
+    for c in calls:
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            outs.append(call(p))
+            outs.append(c())
         graphs.append(g)
-    for k in range(4):
-        for i in (0, 1):
+    for k in range(3):
+        for i, g in enumerate(graphs):
             for t in outs[i]:
                 t.zero_()
-            graphs[i].replay()
-            call(probs[1 - i])
+            g.replay()
+            calls[(i + 1) % len(calls)]()
             torch.cuda.synchronize()
-            assert all(torch.equal(u, v) for u, v in zip(outs[i], want[i])), (k, i)
+            assert same(outs[i], want[i]), (k, i)
