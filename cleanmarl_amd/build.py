@@ -7,12 +7,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcleanmarl_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 out of ordinary float code.  Some of their forms have given wrong results on this hardware now and
-# then; without them the same sums round the same way and an iteration of the 4096-env workload takes 7.73 instead of 7.68 ms.
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Wno-pass-failed",
-         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Wno-pass-failed"]
 INCREMENTAL = False  # set by `python -m cleanmarl_amd.build -i` (development loop); __graft_entry__.build() always compiles everything
-FILE_FLAGS = {}  # per-file extra flags (none: the wave-private actor probe that needed some lives in tools/probes/actor16/)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]  # no v_pk_{add,mul,fma}_f32 from ordinary float code
+FILE_FLAGS = {f"cm_{n}.hip": NO_PACKED_FP32 for n in ("token", "token_f32", "token_f16", "token_bf16", "adamw")}  # per-file extra flags
 
 
 def sources():
