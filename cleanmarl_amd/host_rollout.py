@@ -3,12 +3,14 @@
 The reference exchanges one pickled message per env and step and collates Python lists into padded tensors at the end of the
 episode (cleanmarl/mappo_multienvs.py:393-453, 109-157); `driver.host_rollout_shm` already batches the exchange through shared
 memory but still stages every step through pageable numpy copies (obs -> torch -> .to(device), actions .cpu()) and builds the batch
-on the host.  Here the shared blocks the env workers write (obs, state, availability) and read (actions) are page-locked ONCE
-(hipHostRegister through torch's cudart binding), and a step is
+on the host.  Here each shared block the env workers write (obs, state, availability) or read (actions) has a page-locked twin, allocated ONCE
+(registering the shared memory itself would save the host-side copy, but not every driver allows hipHostRegister on memory it did not
+allocate, and the error of a refused registration is reported by whatever GPU call comes next), and a step is
 
-    3 async H2D copies  shm -> rollout buffer [E, A, t, :]   (the buffer of learner.DeviceBatch, written in place)
+    3 host copies       shm -> page-locked twin
+    3 async H2D copies  twin -> rollout buffer [E, A, t, :]   (the buffer of learner.DeviceBatch, written in place)
     1 act kernel        reads the step's rows of the buffer in place (row stride T), writes action / log-prob in place
-    1 async D2H copy    actions -> the workers' shared action block, 1 stream synchronise, 1 token per worker
+    1 async D2H copy    actions -> twin -> the workers' shared action block, 1 stream synchronise, 1 token per worker
 
 -- no per-step allocation, no pageable copy, no collation: when the last env finishes the batch is already on the device in the
 learner's layout; padded steps of shorter episodes are zeroed by four masked device ops (the reference zero-pads, :113-132).
@@ -20,20 +22,6 @@ from . import _native as N
 from .learner import DeviceBatch
 
 
-def _pin(arr):
-    """Page-lock a numpy array's memory in place (hipHostRegister).  Returns True when the block is pinned."""
-    rt = torch.cuda.cudart()
-    rc = rt.cudaHostRegister(arr.ctypes.data, arr.nbytes, 0)
-    return int(rc) == 0
-
-
-def _unpin(arr):
-    try:
-        torch.cuda.cudart().cudaHostUnregister(arr.ctypes.data)
-    except Exception:  # interpreter shutdown
-        pass
-
-
 class PinnedHostRollout:
     """One episode per env from a `ShmVectorEnv`, written straight into a device-resident DeviceBatch."""
 
@@ -43,11 +31,9 @@ class PinnedHostRollout:
         self.E, self.A, self.Do, self.Ds, self.K = venv.E, venv.A, venv.Do, venv.Ds, venv.K
         self.row_offset = int(row_offset)
         a = venv.arr
-        self.pinned = all([_pin(a[k]) for k in ("obs", "state", "avail", "actions")])
-        if not self.pinned:
-            raise N.NativeError("hipHostRegister of the shared env blocks failed: use --vector_env=shm (host-staged copies)")
-        self.h_obs, self.h_state = torch.from_numpy(a["obs"]), torch.from_numpy(a["state"])
-        self.h_avail, self.h_act = torch.from_numpy(a["avail"]), torch.from_numpy(a["actions"])
+        self.s_obs, self.s_state, self.s_avail, self.s_act = (torch.from_numpy(a[k]) for k in ("obs", "state", "avail", "actions"))
+        self.h_obs, self.h_state, self.h_avail, self.h_act = (torch.empty(t.shape, dtype=t.dtype, pin_memory=True)
+                                                              for t in (self.s_obs, self.s_state, self.s_avail, self.s_act))
         self.cap = int(t_cap)
         # leading dimensions rounded up to 4 floats for the MLP learners' 16-byte tile loads; the GRU / COMA kernels read contiguous rows
         self.pad = (not recurrent) if pad is None else bool(pad)
@@ -57,10 +43,8 @@ class PinnedHostRollout:
         self.calls = 0
 
     def close(self):
-        if self.pinned:
-            for k in ("obs", "state", "avail", "actions"):
-                _unpin(self.v.arr[k])
-            self.pinned = False
+        """The shared blocks belong to the vector env; lets go of the views of them."""
+        self.s_obs = self.s_state = self.s_avail = self.s_act = None
 
     def _grow(self):
         old, T0 = self.buf, self.cap
@@ -109,12 +93,15 @@ class PinnedHostRollout:
                 self._grow()
                 rew = np.concatenate([rew, np.zeros_like(rew)], axis=1)
             b = self.buf
+            for h, shared in ((self.h_obs, self.s_obs), (self.h_state, self.s_state), (self.h_avail, self.s_avail)):
+                h.copy_(shared)
             b.obs[:, :, t].copy_(self.h_obs, non_blocking=True)
             b.state[:, t].copy_(self.h_state, non_blocking=True)
             b.avail[:, :, t].copy_(self.h_avail, non_blocking=True)
             self._act(t, seed, eps)
             self.h_act.copy_(b.action[:, :, t], non_blocking=True)
-            stream.synchronize()  # the workers need the actions; this also fences the H2D copies before the blocks are rewritten
+            stream.synchronize()  # the workers need the actions; this also fences the H2D copies before the twins are rewritten
+            self.s_act.copy_(self.h_act)
             for infos in v._all("step"):
                 if infos:
                     for e, info in infos.items():
