@@ -154,8 +154,9 @@ inline size_t tok_elem(int dtype) { return dtype == CM_DTYPE_F32 ? 4 : 2; }
 constexpr size_t tok_up(size_t n) { return (n + 255) & ~(size_t)255; }
 constexpr size_t TOK_PART_BYTES = (size_t)TOK_MAX_GRID * TOK_STATS * sizeof(double);
 
-size_t tok_scratch(int64_t rows) {  // an order of many rows or the partial sums of few
-    return rows <= TOK_SPLIT_ROWS ? tok_up(TOK_SPLIT_BYTES) : rows <= TOK_ORDER_ROWS ? tok_up((size_t)rows * sizeof(int32_t)) : 0;
+size_t tok_scratch(int64_t rows) {  // an order of many rows or the partial sums of few; never less for more rows
+    const size_t order = tok_up((size_t)(rows < TOK_ORDER_ROWS ? rows : TOK_ORDER_ROWS) * sizeof(int32_t));
+    return order > tok_up(TOK_SPLIT_BYTES) ? order : tok_up(TOK_SPLIT_BYTES);
 }
 int tok_check(const char* who, const cm_token_rows_t* t) {
     CM_REQUIRE(t, "%s: NULL cm_token_rows_t", who);

@@ -56,7 +56,7 @@ enum {
 enum { CM_OPT_ADAM = 0, CM_OPT_ADAMW = 1, CM_OPT_SGD = 2, CM_OPT_RMSPROP = 3 };  /* RMSprop: beta2 := alpha (torch default 0.99) */
 
 const char* cm_last_error(void);
-int cm_version(void);  /* 101 since round 5 (cm_opt_step_t grew by stats_out; cm_optimizer_step_peer takes timeout_s / status; cm_clock_probe) */
+int cm_version(void);  /* 102: cm_token_*, cm_preference_*, cm_adamw_*; 101 since round 5 (cm_opt_step_t grew by stats_out; cm_optimizer_step_peer takes timeout_s / status; cm_clock_probe) */
 /* Schedule / arithmetic options.  The library picks schedules from the problem size (thresholds measured on MI355X);
  * a caller can force one -- for A/B measurements, tests, or a box where the thresholds sit elsewhere.  The library never reads the
  * process environment.  Options are process-wide, take effect at the next launch and may be changed at any time
