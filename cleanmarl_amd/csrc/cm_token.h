@@ -370,16 +370,13 @@ struct TokArgs {
     const float2* keep_in; const float *entropy_in, *d_logp, *d_entropy;     // backward
     void* dlogits; int64_t dld;
     const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy
-    float4* split; int segs; float *g_out, *h_out;                            // few long rows: partial sums (M, s, u, token's logit) of segs segments a row
-    const int32_t* order; unsigned peel;                                      // long rows: the order in which they are taken, NULL: as they are
+    float4* split; int segs;                                                 // few long rows: partial sums (M, s, u, token's logit) of segs segments a row
+    unsigned peel;                                                           // long rows: tok_shape
     const int32_t* range_lo; const int32_t* range_hi;                        // preference: only the rows [*range_lo, *range_hi) are touched
 };
-constexpr int TOK_ORDER_ROWS = 1 << 18;                       // the most rows that are put in order
-constexpr int TOK_SPLIT_ROWS = 256, TOK_SPLIT_SEGS = 32;      // the most rows that are split, the most segments of one
-constexpr size_t TOK_SPLIT_BYTES = TOK_SPLIT_ROWS * (TOK_SPLIT_SEGS * sizeof(float4) + sizeof(float2) + 3 * sizeof(float));
-// (rows that count first, the others behind them: cm_token.hip)
-int tok_launch_order(const TokArgs& a, int32_t* order, hipStream_t s);
-// launches the kernels of one type; `scratch`: room for an order or for partial sums (NULL: neither); returns the number of partial rows of statistics (TOK_POLICY)
+constexpr int TOK_SPLIT_ROWS = 64, TOK_SPLIT_SEGS = 32;  // the most rows that are split, the most segments of one
+constexpr size_t TOK_SPLIT_BYTES = (size_t)TOK_SPLIT_ROWS * TOK_SPLIT_SEGS * sizeof(float4);
+// launches the kernels of one type; `scratch`: TOK_SPLIT_BYTES for partial sums (TOK_LOGP); returns the number of partial rows of statistics (TOK_POLICY)
 int tok_launch_f32(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);
 int tok_launch_f16(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);
 int tok_launch_bf16(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);

@@ -34,66 +34,6 @@ __global__ __launch_bounds__(1024) void k_tok_stats(const double* __restrict__ p
     }
 }
 
-// order[0 .. n): the rows that count, in their order, then the others.  One workgroup: 8192 rows at a time, row 1024 k + thread, so that loads
-// and stores are in order too (a run of rows per thread asked for a cache line per lane: 20 us for 8192 rows); where row r goes follows from the
-// ballots in front of it.
-__global__ __launch_bounds__(1024) void k_tok_order(const void* __restrict__ token, int token_bytes, const float* __restrict__ weight, int rows, int32_t* __restrict__ order) {
-    constexpr int STEPS = 8, CHUNK = 1024 * STEPS;
-    __shared__ int waves[STEPS * 16], all[2];
-    const int32_t* sign = reinterpret_cast<const int32_t*>(token) + (token_bytes == 8 ? 1 : 0);  // the word that holds it
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    unsigned bits = 0;
-    auto look = [&](int r0) {
-        bits = 0;
-#pragma unroll
-        for (int q = 0; q < STEPS; ++q) {
-            const int r = r0 + q * 1024 + (int)threadIdx.x, at = min(r, rows - 1);
-            const int32_t t = sign[(int64_t)at * (token_bytes / 4)];
-            const float w = weight ? weight[at] : 1.0f;
-            bits |= ((r < rows) & (t >= 0) & (w != 0.0f) ? 1u : 0u) << q;
-        }
-    };
-    if (threadIdx.x < 2) all[threadIdx.x] = 0;
-    __syncthreads();
-    for (int r0 = 0; r0 < rows; r0 += CHUNK) {  // how many count at all
-        look(r0);
-        int n = 0;
-#pragma unroll
-        for (int q = 0; q < STEPS; ++q) n += __popcll(__ballot(bits >> q & 1u));
-        if (lane == 0) atomicAdd(&all[0], n);  // whole numbers: any order
-    }
-    __syncthreads();
-    const int total = all[0];
-    int base = 0;  // rows in front of this chunk that count
-    for (int r0 = 0; r0 < rows; r0 += CHUNK) {
-        if (rows > CHUNK) look(r0);
-        unsigned long long mask[STEPS];
-#pragma unroll
-        for (int q = 0; q < STEPS; ++q) {
-            mask[q] = __ballot(bits >> q & 1u);
-            if (lane == 0) waves[q * 16 + wave] = __popcll(mask[q]);
-        }
-        __syncthreads();
-        if (wave == 0) {  // exclusive sums of the 128 counts, two to a lane
-            const int c0 = waves[2 * lane], c1 = waves[2 * lane + 1];
-            int upto = c0 + c1;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(upto, o, 64); if (lane >= o) upto += v; }
-            waves[2 * lane] = upto - c0 - c1; waves[2 * lane + 1] = upto - c1;
-            if (lane == 63) all[1] = upto;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < STEPS; ++q) {
-            const int r = r0 + q * 1024 + (int)threadIdx.x;
-            const int before = base + waves[q * 16 + wave] + __popcll(mask[q] & ((1ull << lane) - 1));
-            if (r < rows) order[bits >> q & 1u ? before : total + r - before] = r;
-        }
-        base += all[1];
-        __syncthreads();  // `waves` and `all` are free again
-    }
-}
-
 // One workgroup per pair: log-probabilities of its two sequences (64-bit sums: thousands of terms, and only their difference counts),
 // the margin, the loss and the factor that every row of the two sequences gets.
 struct PrefArgs {
@@ -154,10 +94,6 @@ inline size_t tok_elem(int dtype) { return dtype == CM_DTYPE_F32 ? 4 : 2; }
 constexpr size_t tok_up(size_t n) { return (n + 255) & ~(size_t)255; }
 constexpr size_t TOK_PART_BYTES = (size_t)TOK_MAX_GRID * TOK_STATS * sizeof(double);
 
-size_t tok_scratch(int64_t rows) {  // an order of many rows or the partial sums of few; never less for more rows
-    const size_t order = tok_up((size_t)(rows < TOK_ORDER_ROWS ? rows : TOK_ORDER_ROWS) * sizeof(int32_t));
-    return order > tok_up(TOK_SPLIT_BYTES) ? order : tok_up(TOK_SPLIT_BYTES);
-}
 int tok_check(const char* who, const cm_token_rows_t* t) {
     CM_REQUIRE(t, "%s: NULL cm_token_rows_t", who);
     CM_REQUIRE(t->dtype == CM_DTYPE_F32 || t->dtype == CM_DTYPE_F16 || t->dtype == CM_DTYPE_BF16, "%s: unknown dtype %d", who, (int)t->dtype);
@@ -198,14 +134,9 @@ TokArgs tok_args(const cm_token_rows_t* t) {
 
 }  // namespace
 
-int tok_launch_order(const TokArgs& a, int32_t* order, hipStream_t s) {
-    hipLaunchKernelGGL(k_tok_order, dim3(1), dim3(1024), 0, s, a.token, a.token_bytes, a.weight, (int)a.rows, order);
-    return 0;
-}
-
 extern "C" size_t cm_token_workspace_bytes(int64_t rows, int vocab) {
     if (rows < 0 || vocab < 1) return 0;
-    return TOK_PART_BYTES + tok_scratch(rows);
+    return TOK_PART_BYTES > TOK_SPLIT_BYTES ? TOK_PART_BYTES : TOK_SPLIT_BYTES;  // a call needs one or the other
 }
 
 extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* entropy, float* keep, void* ws, size_t ws_bytes, cm_stream_t stream) {
@@ -216,7 +147,7 @@ extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* en
     CM_REQUIRE(ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "cm_token_logprob: workspace too small (%zu < %zu) or not 16-byte aligned", ws_bytes, need);
     TokArgs a = tok_args(t);
     a.logp = logp; a.entropy = entropy; a.keep = (float2*)keep;
-    tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, (char*)ws + TOK_PART_BYTES, (hipStream_t)stream);
+    tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, ws, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_logprob");
     return 0;
 }
@@ -250,7 +181,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
     a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws;
-    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, (char*)ws + TOK_PART_BYTES, (hipStream_t)stream);
+    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, nullptr, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd");
     hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(1024), 0, (hipStream_t)stream, a.part, parts, stats);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd/stats");
@@ -260,7 +191,8 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
 extern "C" size_t cm_preference_workspace_bytes(int64_t rows, int vocab, int pairs) {
     if (rows < 0 || vocab < 1 || pairs < 1) return 0;
     return tok_up((size_t)rows * sizeof(float2)) + tok_up((size_t)rows * sizeof(double)) + tok_up((size_t)rows * sizeof(float)) +
-           tok_up((size_t)pairs * TOK_STATS * sizeof(double)) + tok_scratch(rows);
+           tok_up((size_t)pairs * TOK_STATS * sizeof(double)) +
+           tok_up(TOK_SPLIT_BYTES);
 }
 
 extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* seq_start, int pairs, const float* logp_ref, double beta,

@@ -210,7 +210,7 @@ __global__ __launch_bounds__(NT) void k_tok_part(const TokArgs a) {
     const int tid = threadIdx.x, seg = blockIdx.x;
     const int64_t r = blockIdx.y;
     const int64_t tok = tok_in_range(a, r) ? tok_token(a, r) : -1;
-    if (tok < 0 || (a.weight && a.weight[r] == 0.0f)) return;  // k_tok_join does not look at it either
+    if (tok < 0) return;  // k_tok_join does not look at it either
     const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
     const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
     const TokShape shape = tok_shape<T>(row, a.V, a.peel);
@@ -230,77 +230,52 @@ __global__ __launch_bounds__(NT) void k_tok_part(const TokArgs a) {
     if (tid == 0) a.split[r * a.segs + seg] = make_float4(z.M, z.s, z.u, seg == 0 ? tok_logit<T, AV>(row, av, tok, a.V) : 0.0f);
 }
 
-// Half a wave per row and round.  TOK_POLICY: one workgroup, which adds up the statistics as well and leaves to k_tok_back what it needs of each row.
-template <class T, int MODE, bool AV, bool EN, int NT>
+// Half a wave per row.
+template <class T, bool AV, bool EN, int NT>
 __global__ __launch_bounds__(NT) void k_tok_join(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int PER = NT / 32;
-    constexpr bool ENT = EN || MODE == TOK_POLICY;
     __shared__ TokSum careful[NT / 64], sums[PER];
     __shared__ int odd[PER];
-    __shared__ double sh[NT / 64][TOK_STATS];
     const int lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
-    double st[TOK_STATS] = {};
-    for (int64_t r0 = (int64_t)blockIdx.x * PER; r0 < a.rows; r0 += (int64_t)gridDim.x * PER) {
-        const int64_t r = r0 + slot;
-        const bool here = r < a.rows && tok_in_range(a, r);
-        const int64_t tok = here ? tok_token(a, r) : -1;
-        TokPolicyRow q = {};
-        if (MODE == TOK_POLICY && here) q = tok_policy_load(a, r);
-        const bool counts = tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f);
-        TokRun z = {TOK_START, 0.0f, 0.0f};
-        float x = 0.0f;
-        if (counts) {
-            const float4 v = lane < a.segs ? a.split[r * a.segs + lane] : make_float4(TOK_START, 0.0f, 0.0f, 0.0f);
-            z = {v.x, v.y, v.z};
-            x = __shfl(v.w, threadIdx.x & 32, 64);
-            run_group<ENT, 32>(z);
-        }
-        const bool ordinary = run_ordinary<ENT>(z);
-        if (lane == 0) odd[slot] = counts && !ordinary;
-        __syncthreads();
-        for (int p = 0; p < PER; ++p) {  // rows that have to be done over, by all
-            if (!odd[p]) continue;
-            const TokSum y = tok_careful_sum<T, AV, ENT, NT>(reinterpret_cast<const elem*>(a.logits) + (r0 + p) * a.ld, AV ? a.avail + (r0 + p) * a.avail_ld : nullptr, a, careful);
-            if (threadIdx.x == 0) sums[p] = y;
-            __syncthreads();
-        }
-        if (here && lane == 0) {
-            float logp = 0.0f, H = 0.0f, g = 0.0f, h = 0.0f;
-            double logp64 = 0.0;
-            float2 keep = {0.0f, 0.0f};
-            if (counts) {
-                const TokSum y = ordinary ? TokSum{0.0f, z.s, z.u} : sums[slot];
-                const float logs = logf(y.s);
-                if (y.s != 0.0f) {
-                    logp = ordinary ? run_logp(x, z.M, logs, a.c) : tok_logp(x, y.m, logs, a.c);
-                    if (ENT) H = logs - y.u / y.s * TOK_LN2;
-                    if (MODE == TOK_POLICY) tok_policy_row(a, q, logp, H, true, st, g, h);
-                }
-                keep = ordinary ? make_float2(z.M, -run_sum(z, a.c)) : make_float2(y.m, y.s);
-                logp64 = ordinary ? run_logp64(x, z.M, z.s, a.c) : tok_logp64(x, y.m, y.s, a.c);
-            }
-            if (a.logp) a.logp[r] = logp;
-            if (a.logp64) a.logp64[r] = logp64;
-            if (a.keep) a.keep[r] = keep;
-            if (ENT && a.entropy) a.entropy[r] = H;
-            if (MODE == TOK_POLICY) { a.g_out[r] = g; a.h_out[r] = -h; }
-        }
-        __syncthreads();  // odd, sums, careful are free again
+    const int64_t r0 = (int64_t)blockIdx.x * PER, r = r0 + slot;
+    const bool here = r < a.rows && tok_in_range(a, r);
+    const bool counts = here && tok_token(a, r) >= 0;
+    TokRun z = {TOK_START, 0.0f, 0.0f};
+    float x = 0.0f;
+    if (counts) {
+        const float4 v = lane < a.segs ? a.split[r * a.segs + lane] : make_float4(TOK_START, 0.0f, 0.0f, 0.0f);
+        z = {v.x, v.y, v.z};
+        x = __shfl(v.w, threadIdx.x & 32, 64);
+        run_group<EN, 32>(z);
     }
-    if (MODE == TOK_POLICY) {
-#pragma unroll
-        for (int i = 0; i < TOK_STATS; ++i) {
-            const double v = cm_wave_sum_d(st[i]);
-            if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6][i] = v;
-        }
+    const bool ordinary = run_ordinary<EN>(z);
+    if (lane == 0) odd[slot] = counts && !ordinary;
+    __syncthreads();
+    for (int p = 0; p < PER; ++p) {  // rows that have to be done over, by all
+        if (!odd[p]) continue;
+        const TokSum y = tok_careful_sum<T, AV, EN, NT>(reinterpret_cast<const elem*>(a.logits) + (r0 + p) * a.ld, AV ? a.avail + (r0 + p) * a.avail_ld : nullptr, a, careful);
+        if (threadIdx.x == 0) sums[p] = y;
         __syncthreads();
-        if (threadIdx.x < TOK_STATS) {
-            double v = 0.0;
-            for (int w = 0; w < NT / 64; ++w) v += sh[w][threadIdx.x];
-            a.part[threadIdx.x] = v;
-        }
     }
+    if (!here || lane != 0) return;
+    float logp = 0.0f, H = 0.0f;
+    double logp64 = 0.0;
+    float2 keep = {0.0f, 0.0f};
+    if (counts) {
+        const TokSum y = ordinary ? TokSum{0.0f, z.s, z.u} : sums[slot];
+        const float logs = logf(y.s);
+        if (y.s != 0.0f) {
+            logp = ordinary ? run_logp(x, z.M, logs, a.c) : tok_logp(x, y.m, logs, a.c);
+            if (EN) H = logs - y.u / y.s * TOK_LN2;
+        }
+        keep = ordinary ? make_float2(z.M, -run_sum(z, a.c)) : make_float2(y.m, y.s);
+        logp64 = ordinary ? run_logp64(x, z.M, z.s, a.c) : tok_logp64(x, y.m, y.s, a.c);
+    }
+    if (a.logp) a.logp[r] = logp;
+    if (a.logp64) a.logp64[r] = logp64;
+    if (a.keep) a.keep[r] = keep;
+    if (EN && a.entropy) a.entropy[r] = H;
 }
 
 // Backward only, rows too long for a wave: nothing is summed, so a workgroup takes NT * U pieces of one row, whichever.  The rows come in
@@ -388,7 +363,7 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
 // Short rows: G lanes of a wave hold one row in registers (NV pieces of 16 bytes to a lane), 64 / G rows to a wave.  The row is read once,
 // its exponentials are made once and scaled into the gradient.
 template <class T, int MODE, bool AV, bool EN, int G, int NV>
-__global__ __launch_bounds__(256, 8) void k_tok_short(const TokArgs a) {
+__global__ __launch_bounds__(256, NV * G < 256 ? 8 : NV == 4 ? 5 : 4) void k_tok_short(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, PER = 256 / G;
     constexpr bool ENT = EN || MODE == TOK_POLICY;
@@ -505,16 +480,15 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
     int turn = 0;
     const int tid = threadIdx.x;
     struct Row { int64_t tok; TokPolicyRow q; bool live; };
-    auto scalars = [&](int64_t r, bool there) {
+    auto scalars = [&](int64_t r) {
         Row s = {-1, {}, false};
-        if (there) {
+        if (r < a.rows) {
             s.tok = a.token_bytes == 8 ? tok_scalar((const int64_t*)a.token, r) : (int64_t)tok_scalar((const int32_t*)a.token, r);
             s.q = {tok_scalar(a.logp_old, r), tok_scalar(a.adv, r), a.logp_ref ? tok_scalar(a.logp_ref, r) : 0.0f, a.weight ? tok_scalar(a.weight, r) : 1.0f};
             s.live = s.tok >= 0 && s.q.w != 0.0f;
         }
         return s;
     };
-    auto index = [&](int64_t i) -> int64_t { return a.order && i < a.rows ? tok_scalar(a.order, i) : i; };
     auto row_at = [&](int64_t r) { return reinterpret_cast<const elem*>(a.logits) + r * a.ld; };
     auto drow_at = [&](int64_t r) { return reinterpret_cast<elem*>(a.dlogits) + r * a.dld; };
     auto av_at = [&](int64_t r) { return AV ? a.avail + r * a.avail_ld : nullptr; };
@@ -558,13 +532,13 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
             }
         }
     };
-    int64_t i = blockIdx.x, r = index(i);
-    Row now = scalars(r, true);
+    int64_t r = blockIdx.x;
+    Row now = scalars(r);
     TokShape shape = tok_shape<T>(drow_at(r), a.V, a.peel);
     fill(row_at(r), av_at(r), shape);
-    for (; i < a.rows; i += gridDim.x) {
-        const int64_t rn = index(i + gridDim.x);
-        const Row next = scalars(rn, i + gridDim.x < a.rows);
+    for (; r < a.rows; r += gridDim.x) {
+        const int64_t rn = r + gridDim.x;
+        const Row next = scalars(rn);
         const elem *row = row_at(r), *nrow = next.live ? row_at(rn) : row;
         const uint8_t *av = av_at(r), *nav = next.live ? av_at(rn) : av;
         const TokShape nshape = tok_shape<T>(drow_at(rn), a.V, a.peel);
@@ -661,7 +635,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
                 fill(nrow, nav, nshape);
             }
         }
-        now = next; r = rn; shape = nshape;
+        now = next; shape = nshape;
     }
     if (tid == 0)
         for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
@@ -679,31 +653,27 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
     if (nvec <= 8) TOK_SHORT(4, 2);
     if (nvec <= 32) TOK_SHORT(16, 2);
     if (nvec <= 128) TOK_SHORT(64, 2);
+    if (nvec <= 256) TOK_SHORT(64, 4);
+    if (nvec <= 512) TOK_SHORT(64, 8);
 #undef TOK_SHORT
     const int64_t nfull = a.V / T::W;
-    auto back = [&](const TokArgs& b) {
-        constexpr int NT = 256, U = 4;
-        const int parts = (int)((nfull + NT * U - 1) / (NT * U));
-        const int64_t tiles = b.rows * parts;
-        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, b, parts, tiles);
-    };
     a.peel = 127u;
     if constexpr (MODE == TOK_BWD) {
-        back(a);
+        constexpr int NT = 256, U = 4;
+        const int parts = (int)((nfull + NT * U - 1) / (NT * U));
+        const int64_t tiles = a.rows * parts;
+        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, a, parts, tiles);
         return 0;
     }
-    // few long rows: enough segments for some 1024 workgroups, at least 512 pieces (8 KB) in each
-    const int64_t most = 1024 / a.rows < nfull / 512 ? 1024 / a.rows : nfull / 512;
-    a.segs = (int)(most < TOK_SPLIT_SEGS ? most : TOK_SPLIT_SEGS);
-    const bool split = scratch && a.rows <= TOK_SPLIT_ROWS && a.segs >= 2;
-    if (split) {
-        a.split = reinterpret_cast<float4*>(scratch);
-        a.peel = 127u;
-    }
     if constexpr (MODE == TOK_LOGP) {
-        if (split) {
+        // Few long rows in segments of at least 512 pieces (8 KB).  GPU time, bf16: 16 rows of 131072 columns 14.2 -> 7.7 us, 64 rows 14.8 -> 11.1; but
+        // 128 rows of 65536 9.3 -> 11.0, 64 rows of 16384 4.5 -> 7.5: below 8192 pieces a row is done before a second launch has begun.
+        if (a.rows <= TOK_SPLIT_ROWS && nfull >= 8192) {
+            const int64_t most = 1024 / a.rows < nfull / 512 ? 1024 / a.rows : nfull / 512;
+            a.segs = (int)(most < TOK_SPLIT_SEGS ? most : TOK_SPLIT_SEGS);
+            a.split = reinterpret_cast<float4*>(scratch);
             hipLaunchKernelGGL((k_tok_part<T, AV, EN, 256>), dim3(a.segs, (unsigned)a.rows), dim3(256), 0, s, a);
-            hipLaunchKernelGGL((k_tok_join<T, MODE, AV, EN, 256>), dim3((unsigned)(a.rows + 7) / 8), dim3(256), 0, s, a);
+            hipLaunchKernelGGL((k_tok_join<T, AV, EN, 256>), dim3((unsigned)(a.rows + 7) / 8), dim3(256), 0, s, a);
             return 0;
         }
         const int grid = (int)(a.rows < (1 << 20) ? a.rows : (1 << 20));
@@ -711,29 +681,10 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
         return grid;
     }
     if constexpr (MODE == TOK_POLICY) {
-        // a third launch instead of one sweep of whole rows: from rows on that keep a workgroup busy for some 10 us
-        if (split && a.rows <= 64 && nfull > 512 * 12) {
-            a.keep = reinterpret_cast<float2*>(a.split + TOK_SPLIT_ROWS * TOK_SPLIT_SEGS);
-            a.g_out = reinterpret_cast<float*>(a.keep + TOK_SPLIT_ROWS); a.h_out = a.g_out + TOK_SPLIT_ROWS; a.entropy = a.h_out + TOK_SPLIT_ROWS;
-            hipLaunchKernelGGL((k_tok_part<T, AV, true, 256>), dim3(a.segs, (unsigned)a.rows), dim3(256), 0, s, a);
-            hipLaunchKernelGGL((k_tok_join<T, MODE, AV, EN, 1024>), dim3(1), dim3(1024), 0, s, a);
-            TokArgs b = a;
-            b.keep_in = a.keep; b.entropy_in = a.entropy; b.d_logp = a.g_out; b.d_entropy = a.h_out;
-            back(b);
-            return 1;
-        }
         constexpr int HEAD = (128 / (int)sizeof(typename T::elem) + T::W - 1) / T::W;  // the most pieces that a head takes from the body
         // FULL pieces of every thread exist: nfull > NT * FULL; a head is only peeled off where they still do
-        // Rows that are left out (prompts, padding) cost next to nothing and come in patterns: without an order some workgroups would get few of
-        // them (3001 x 100003 fp16, 30 % left out: 430 -> 330 us).  The order costs a launch and 5 us for 8192 rows: worth it from some 50 us on.
-        auto in_order = [&](int grid) {
-            if (scratch && a.rows > grid && a.rows <= TOK_ORDER_ROWS && a.rows * a.V >= (int64_t)1 << 26) {
-                tok_launch_order(a, reinterpret_cast<int32_t*>(scratch), s);
-                a.order = reinterpret_cast<const int32_t*>(scratch);
-            }
-        };
 #define TOK_REGS(NT, NV, FULL, PER_CU) do { if (nfull <= NT * NV) { const int grid = (int)(a.rows < 256 * PER_CU ? a.rows : 256 * PER_CU); \
-        a.peel = nfull - HEAD >= NT * FULL ? 127u : 0u; in_order(grid); \
+        a.peel = nfull - HEAD >= NT * FULL ? 127u : 0u; \
         hipLaunchKernelGGL((k_tok_regs<T, AV, EN, NT, NV, FULL>), dim3(grid), dim3(NT), 0, s, a); return grid; } } while (0)
         TOK_REGS(256, 4, 0, 8);
         TOK_REGS(256, 8, 4, 4);

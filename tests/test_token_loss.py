@@ -411,9 +411,9 @@ def test_policy_loss_on_rows_of_every_size(V, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("V, dtype", [(65536, torch.bfloat16), (32768, torch.float32), (65601, torch.float16)])
-def test_rows_that_count_come_first(V, dtype):
-    """Long batches are taken in the order of the rows that count.  The same rows in slices, each too short for an order, give the same values: bit by bit where
-    every row starts at the same alignment, else within the bars of both (twice one bar)."""
+def test_a_long_batch_in_slices(V, dtype):
+    """More rows than workgroups, some left out: the same rows in slices of less than one round give the same values, bit by bit where every row starts at the
+    same alignment, else within the bars of both (twice one bar)."""
     from cleanmarl_amd import token_loss as TL
     rows = 2300 if V % 64 == 0 else 1100
     gen = torch.Generator("cuda").manual_seed(V)
