@@ -372,10 +372,36 @@ struct TokArgs {
     const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy
     float4* split; int segs;                                                 // few long rows: partial sums (M, s, u, token's logit) of segs segments a row
     unsigned peel;                                                           // long rows: tok_shape
+    float* stats;                                                            // policy: where a launch of one workgroup writes its sums; preference: see pairs
+    const double* pair_part; int pairs;                                      // preference, backward: the first workgroup adds up what k_pref_pair left of each pair
     const int32_t* range_lo; const int32_t* range_hi;                        // preference: only the rows [*range_lo, *range_hi) are touched
 };
 constexpr int TOK_SPLIT_ROWS = 64, TOK_SPLIT_SEGS = 32;  // the most rows that are split, the most segments of one
 constexpr size_t TOK_SPLIT_BYTES = (size_t)TOK_SPLIT_ROWS * TOK_SPLIT_SEGS * sizeof(float4);
+// sums of n partial rows of statistics in a fixed order, by a workgroup of NT threads (one call per kernel)
+template <int NT>
+__device__ __forceinline__ void tok_sum_stats(const double* part, int n, float* stats) {
+    constexpr int GROUPS = NT / TOK_STATS, BATCH = 8;
+    __shared__ double sh[NT / 64][TOK_STATS];
+    const int c = threadIdx.x % TOK_STATS, g = threadIdx.x / TOK_STATS;
+    double s = 0.0;
+    for (int i0 = g; i0 < n; i0 += GROUPS * BATCH) {  // a batch of loads in flight
+        double v[BATCH];
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) v[q] = i0 + q * GROUPS < n ? part[(int64_t)(i0 + q * GROUPS) * TOK_STATS + c] : 0.0;
+#pragma unroll
+        for (int q = 0; q < BATCH; ++q) s += v[q];
+    }
+#pragma unroll
+    for (int o = 32; o >= TOK_STATS; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) < TOK_STATS) sh[threadIdx.x >> 6][c] = s;
+    __syncthreads();
+    if (threadIdx.x < TOK_STATS) {
+        double t = 0.0;
+        for (int i = 0; i < NT / 64; ++i) t += sh[i][c];
+        stats[c] = (float)t;
+    }
+}
 // launches the kernels of one type; `scratch`: TOK_SPLIT_BYTES for partial sums (TOK_LOGP); returns the number of partial rows of statistics (TOK_POLICY)
 int tok_launch_f32(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);
 int tok_launch_f16(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);

@@ -10,29 +10,7 @@
 
 namespace {
 
-// sums of n partial rows of statistics, in a fixed order
-__global__ __launch_bounds__(1024) void k_tok_stats(const double* __restrict__ part, int n, float* __restrict__ stats) {
-    constexpr int GROUPS = 1024 / TOK_STATS, BATCH = 8;
-    __shared__ double sh[16][TOK_STATS];
-    const int c = threadIdx.x % TOK_STATS, g = threadIdx.x / TOK_STATS;
-    double s = 0.0;
-    for (int i0 = g; i0 < n; i0 += GROUPS * BATCH) {
-        double v[BATCH];
-#pragma unroll
-        for (int q = 0; q < BATCH; ++q) v[q] = i0 + q * GROUPS < n ? part[(int64_t)(i0 + q * GROUPS) * TOK_STATS + c] : 0.0;
-#pragma unroll
-        for (int q = 0; q < BATCH; ++q) s += v[q];
-    }
-#pragma unroll
-    for (int o = 32; o >= TOK_STATS; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) < TOK_STATS) sh[threadIdx.x >> 6][c] = s;
-    __syncthreads();
-    if (threadIdx.x < TOK_STATS) {
-        double t = 0.0;
-        for (int i = 0; i < 16; ++i) t += sh[i][c];
-        stats[c] = (float)t;
-    }
-}
+__global__ __launch_bounds__(1024) void k_tok_stats(const double* __restrict__ part, int n, float* __restrict__ stats) { tok_sum_stats<1024>(part, n, stats); }
 
 // One workgroup per pair: log-probabilities of its two sequences (64-bit sums: thousands of terms, and only their difference counts),
 // the margin, the loss and the factor that every row of the two sequences gets.
@@ -180,11 +158,13 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     TokArgs a = tok_args(t);
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
-    a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws;
+    a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws; a.stats = stats;
     const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, nullptr, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd");
-    hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(1024), 0, (hipStream_t)stream, a.part, parts, stats);
-    CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd/stats");
+    if (parts != 1) {  // one workgroup has written the sums itself
+        hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(1024), 0, (hipStream_t)stream, a.part, parts, stats);
+        CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd/stats");
+    }
     return 0;
 }
 
@@ -223,9 +203,12 @@ extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* se
     hipLaunchKernelGGL(k_pref_pair, dim3(pairs), dim3(256), 0, s, p);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/pair");
     a.keep_in = keep; a.d_logp = coef; a.dlogits = dlogits; a.dld = dlogits_ld;
+    a.pair_part = part; a.pairs = pairs; a.stats = stats;
     tok_launch(a, t->dtype, TOK_BWD, false, nullptr, s);
     CM_CHECK_LAUNCH("cm_preference_fwd_bwd/bwd");
-    hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(1024), 0, s, part, pairs, stats);
-    CM_CHECK_LAUNCH("cm_preference_fwd_bwd/stats");
+    if (t->rows == 0) {
+        hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(1024), 0, s, part, pairs, stats);
+        CM_CHECK_LAUNCH("cm_preference_fwd_bwd/stats");
+    }
     return 0;
 }

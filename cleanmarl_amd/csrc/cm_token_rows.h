@@ -117,7 +117,7 @@ __global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
         tok_careful_grad<T, AV, EN, NT>(row, av, reinterpret_cast<elem*>(a.dlogits) + r * a.dld, a, g, live);
     }
     if (threadIdx.x == 0)
-        for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
+        for (int i = 0; i < TOK_STATS; ++i) { if (gridDim.x == 1) a.stats[i] = (float)st[i]; else a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i]; }
 }
 
 // Forward only, rows too long for a wave: a workgroup per row, several to a CU, two batches of U pieces to a thread in flight.
@@ -285,6 +285,7 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
     typedef typename T::elem elem;
     constexpr int W = T::W;
     const int tid = threadIdx.x;
+    if (a.pair_part && blockIdx.x == 0) tok_sum_stats<NT>(a.pair_part, a.pairs, a.stats);
     for (int64_t t = tiles - 1 - blockIdx.x; t >= 0; t -= gridDim.x) {
         const int64_t r = t / parts;
         const int part = (int)(t - r * parts);
@@ -368,6 +369,7 @@ __global__ __launch_bounds__(256, NV * G < 256 ? 8 : NV == 4 ? 5 : 4) void k_tok
     constexpr int W = T::W, PER = 256 / G;
     constexpr bool ENT = EN || MODE == TOK_POLICY;
     const int gl = threadIdx.x & (G - 1);  // lane in the group
+    if (MODE == TOK_BWD && a.pair_part && blockIdx.x == 0) tok_sum_stats<256>(a.pair_part, a.pairs, a.stats);
     double st[TOK_STATS] = {};
     for (int64_t r = (int64_t)blockIdx.x * PER + threadIdx.x / G; r < a.rows; r += (int64_t)gridDim.x * PER) {
         if (!tok_in_range(a, r)) continue;
@@ -458,7 +460,10 @@ __global__ __launch_bounds__(256, NV * G < 256 ? 8 : NV == 4 ? 5 : 4) void k_tok
             if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6][i] = v;
         }
         __syncthreads();
-        if (threadIdx.x < TOK_STATS) a.part[(int64_t)blockIdx.x * TOK_STATS + threadIdx.x] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+        if (threadIdx.x < TOK_STATS) {
+            const double v = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+            if (gridDim.x == 1) a.stats[threadIdx.x] = (float)v; else a.part[(int64_t)blockIdx.x * TOK_STATS + threadIdx.x] = v;
+        }
     }
 }
 
@@ -638,7 +643,7 @@ __global__ __launch_bounds__(NT) void k_tok_regs(const TokArgs a) {
         now = next; shape = nshape;
     }
     if (tid == 0)
-        for (int i = 0; i < TOK_STATS; ++i) a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i];
+        for (int i = 0; i < TOK_STATS; ++i) { if (gridDim.x == 1) a.stats[i] = (float)st[i]; else a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i]; }
 }
 
 // ---------------------------------------------------------------- choice of a kernel
@@ -647,7 +652,9 @@ inline int tok_grid(int64_t items) { return (int)(items < TOK_MAX_GRID ? (items 
 template <class T, int MODE, bool AV, bool EN>
 int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
     const int64_t nvec = ((int64_t)a.V + T::W - 1) / T::W;
-#define TOK_SHORT(G, NV) do { const int grid = tok_grid((a.rows + 256 / G - 1) / (256 / G)); \
+    // a policy loss of few rows in one workgroup, up to four rounds of short ones (2 us each): less than a second launch that adds up statistics (4 us); four
+    // rounds of 4096 columns took 23 us
+#define TOK_SHORT(G, NV) do { const int grid = MODE == TOK_POLICY && a.rows <= (G < 64 ? 4 : 1) * (256 / G) ? 1 : tok_grid((a.rows + 256 / G - 1) / (256 / G)); \
         hipLaunchKernelGGL((k_tok_short<T, MODE, AV, EN, G, NV>), dim3(grid), dim3(256), 0, s, a); return grid; } while (0)
     if (nvec <= 2) TOK_SHORT(1, 2);
     if (nvec <= 8) TOK_SHORT(4, 2);

@@ -85,8 +85,8 @@ def _rows(logits, token, avail, temperature):
 def _grad(out, logits):
     """The tensor that receives the gradient and its row stride; ``out`` may be the logits themselves."""
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    elif out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
+        return torch.empty_like(logits, memory_format=torch.contiguous_format), logits.shape[-1]
+    if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
         raise ValueError(f"out: need {logits.dtype} {tuple(logits.shape)} on {logits.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
     return out, _row_stride(out, "out")
 
@@ -145,7 +145,7 @@ def policy_loss_fwd_bwd(logits, token, logp_old, adv, logp_ref=None, weight=None
     with N.on_device(index):
         out, ld = _grad(out, logits)
         stats = torch.empty(N.NUM_STATS, dtype=torch.float32, device=device)
-        logp = torch.empty(token.shape, dtype=torch.float32, device=device)
+        logp = torch.empty_like(logp_old)
         nbytes = lib.cm_token_workspace_bytes(rows.rows, rows.vocab)
         ws = _workspace(nbytes, device)
         N.check(lib.cm_token_policy_fwd_bwd(C.byref(rows), old, ad, ref, w, clip_low, clip_high, kl_coef, entropy_coef, out.data_ptr(), ld, logp.data_ptr(),
