@@ -370,6 +370,7 @@ struct TokArgs {
     const float2* keep_in; const float *entropy_in, *d_logp, *d_entropy;     // backward
     void* dlogits; int64_t dld;
     const float *logp_old, *adv, *logp_ref, *weight; float lo, hi, kl_coef, ent_coef; double* part;  // policy
+    float *g_out, *h_out;                                                    // policy in two launches: the factors of each row for the second
     float4* split; int segs;                                                 // few long rows: partial sums (M, s, u, token's logit) of segs segments a row
     unsigned peel;                                                           // long rows: tok_shape
     float* stats;                                                            // policy: where a launch of one workgroup writes its sums; preference: see pairs
@@ -377,6 +378,8 @@ struct TokArgs {
     const int32_t* range_lo; const int32_t* range_hi;                        // preference: only the rows [*range_lo, *range_hi) are touched
 };
 constexpr int TOK_SPLIT_ROWS = 64, TOK_SPLIT_SEGS = 32;  // the most rows that are split, the most segments of one
+constexpr int TOK_HELD = 1024 * 16 * 16;                 // a policy loss holds rows of up to this many bytes, at least
+constexpr size_t TOK_ROW_BYTES = sizeof(float2) + 3 * sizeof(float);
 constexpr size_t TOK_SPLIT_BYTES = (size_t)TOK_SPLIT_ROWS * TOK_SPLIT_SEGS * sizeof(float4);
 // sums of n partial rows of statistics in a fixed order, by a workgroup of NT threads (one call per kernel)
 template <int NT>
@@ -402,7 +405,8 @@ __device__ __forceinline__ void tok_sum_stats(const double* part, int n, float* 
         stats[c] = (float)t;
     }
 }
-// launches the kernels of one type; `scratch`: TOK_SPLIT_BYTES for partial sums (TOK_LOGP); returns the number of partial rows of statistics (TOK_POLICY)
+// launches the kernels of one type; `scratch`: TOK_SPLIT_BYTES for partial sums (TOK_LOGP), TOK_ROW_BYTES a row (TOK_POLICY, more than
+// TOK_HELD bytes of logits); returns the number of partial rows of statistics (TOK_POLICY)
 int tok_launch_f32(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);
 int tok_launch_f16(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);
 int tok_launch_bf16(TokArgs a, int mode, bool en, void* scratch, hipStream_t s);

@@ -114,7 +114,8 @@ TokArgs tok_args(const cm_token_rows_t* t) {
 
 extern "C" size_t cm_token_workspace_bytes(int64_t rows, int vocab) {
     if (rows < 0 || vocab < 1) return 0;
-    return TOK_PART_BYTES > TOK_SPLIT_BYTES ? TOK_PART_BYTES : TOK_SPLIT_BYTES;  // a call needs one or the other
+    static_assert(TOK_PART_BYTES >= TOK_SPLIT_BYTES, "log-probabilities use the room of the statistics");
+    return TOK_PART_BYTES + (vocab > TOK_HELD / 4 ? tok_up((size_t)rows * TOK_ROW_BYTES) : 0);
 }
 
 extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* entropy, float* keep, void* ws, size_t ws_bytes, cm_stream_t stream) {
@@ -159,7 +160,7 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
     a.dlogits = dlogits; a.dld = dlogits_ld; a.logp = logp; a.part = (double*)ws; a.stats = stats;
-    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, nullptr, (hipStream_t)stream);
+    const int parts = tok_launch(a, t->dtype, TOK_POLICY, entropy_coef != 0.0, t->vocab > TOK_HELD / 4 ? (char*)ws + TOK_PART_BYTES : nullptr, (hipStream_t)stream);
     CM_CHECK_LAUNCH("cm_token_policy_fwd_bwd");
     if (parts != 1) {  // one workgroup has written the sums itself
         hipLaunchKernelGGL(k_tok_stats, dim3(1), dim3(1024), 0, (hipStream_t)stream, a.part, parts, stats);

@@ -81,52 +81,17 @@ __device__ __forceinline__ void tok_careful_grad(const typename T::elem* row, co
     }
 }
 
-// Rows that no workgroup can hold: a workgroup walks a row twice, once for (m, s, u) and once, reading it again (a part of it from a cache), to
-// write the gradient.
-template <class T, bool AV, bool EN, int NT>
-__global__ __launch_bounds__(NT) void k_tok_stream(const TokArgs a) {
-    typedef typename T::elem elem;
-    __shared__ TokSum sh[2][NT / 64];
-    double st[TOK_STATS] = {};
-    int turn = 0;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const elem* row = reinterpret_cast<const elem*>(a.logits) + r * a.ld;
-        const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
-        const int64_t tok = tok_token(a, r);
-        const TokPolicyRow q = tok_policy_load(a, r);
-        bool live = tok >= 0 && q.w != 0.0f;
-        TokGrad g = {};
-        float logp = 0.0f;
-        if (live) {
-            const float x = tok_logit<T, AV>(row, av, tok, a.V);
-            const TokSum z = tok_careful_sum<T, AV, true, NT>(row, av, a, sh[turn]);  // its barrier: all have read the token's logit before a gradient is written over it
-            turn ^= 1;
-            live = z.s != 0.0f;
-            if (live) {
-                const float logs = logf(z.s);
-                g.m = z.m; g.rs = 1.0f / z.s;
-                logp = tok_logp(x, z.m, logs, a.c);
-                g.K = -z.u * g.rs * TOK_LN2;
-                float gg, hh;
-                tok_policy_row(a, q, logp, logs + g.K, threadIdx.x == 0, st, gg, hh);
-                g.a = g.b = gg * a.c.nat; g.h = hh * a.c.nat;
-            }
-        }
-        if (threadIdx.x == 0 && a.logp) a.logp[r] = logp;
-        g.tok = (int)(live && tok < a.V && (!AV || av[tok]) ? tok : -1);  // an unavailable place has no gradient
-        tok_careful_grad<T, AV, EN, NT>(row, av, reinterpret_cast<elem*>(a.dlogits) + r * a.dld, a, g, live);
-    }
-    if (threadIdx.x == 0)
-        for (int i = 0; i < TOK_STATS; ++i) { if (gridDim.x == 1) a.stats[i] = (float)st[i]; else a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i]; }
-}
-
-// Forward only, rows too long for a wave: a workgroup per row, several to a CU, two batches of U pieces to a thread in flight.
-template <class T, bool AV, bool EN, int NT, int U>
+// Forward only, rows too long for a wave: a workgroup per row, several to a CU, two batches of U pieces to a thread in flight (U = 4 holds more in
+// flight and fewer workgroups: 98 us against 90 for 4096 x 50001 fp16 with entropies).  TOK_POLICY: rows that no workgroup can hold; what k_tok_back needs
+// of each goes to memory.
+template <class T, int MODE, bool AV, bool EN, int NT, int U>
 __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
     typedef typename T::elem elem;
     constexpr int W = T::W, NW = NT / 64;
     __shared__ TokRun sh[2][NW];
     __shared__ TokSum careful[NW];
+    __shared__ double st[TOK_STATS];
+    if (MODE == TOK_POLICY && threadIdx.x == 0) for (int i = 0; i < TOK_STATS; ++i) st[i] = 0.0;
     int turn = 0;
     const int tid = threadIdx.x;
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -136,7 +101,9 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
         const uint8_t* av = AV ? a.avail + r * a.avail_ld : nullptr;
         float x = 0.0f, logp = 0.0f, H = 0.0f;
         float2 keep = {0.0f, 0.0f};
-        if (tok >= 0) {
+        TokPolicyRow q = {};
+        if (MODE == TOK_POLICY) q = tok_policy_load(a, r);
+        if (tok >= 0 && (MODE != TOK_POLICY || q.w != 0.0f)) {
             x = tok_logit<T, AV>(row, av, tok, a.V);
             const TokShape shape = tok_shape<T>(row, a.V, a.peel);
             const elem* body = row + shape.head;
@@ -196,9 +163,17 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
             if (a.logp64 && tok < 0) a.logp64[r] = 0.0;
             if (EN && a.entropy) a.entropy[r] = H;
             if (a.keep) a.keep[r] = keep;
+            if (MODE == TOK_POLICY && keep.y != 0.0f) {
+                float g, h;
+                tok_policy_row(a, q, logp, H, true, st, g, h);
+                a.g_out[r] = g; a.h_out[r] = -h;
+            }
         }
     }
+    if (MODE == TOK_POLICY && tid == 0)
+        for (int i = 0; i < TOK_STATS; ++i) { if (gridDim.x == 1) a.stats[i] = (float)st[i]; else a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i]; }
 }
+
 
 // Few long rows: a row is cut into segments, a workgroup sums one, k_tok_join puts them together.  (16 rows of 131072 bf16 columns: 13.3 us with
 // a workgroup per row.)
@@ -279,7 +254,8 @@ __global__ __launch_bounds__(NT) void k_tok_join(const TokArgs a) {
 }
 
 // Backward only, rows too long for a wave: nothing is summed, so a workgroup takes NT * U pieces of one row, whichever.  The rows come in
-// descending order: the last ones that a forward sweep has read are the ones still in a cache.
+// descending order: the last ones that a forward sweep has read are the ones still in a cache.  Stores are streaming ones, they would push the logits
+// out of it (2048 x 32000 fp32, both sweeps: 160 us, so 129).  8192 x 131072 bf16 alone: 0.74 ms, 5.8 TB/s.
 template <class T, bool AV, bool EN, int NT, int U>
 __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int64_t tiles) {
     typedef typename T::elem elem;
@@ -361,8 +337,9 @@ __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int
     }
 }
 
-// Short rows: G lanes of a wave hold one row in registers (NV pieces of 16 bytes to a lane), 64 / G rows to a wave.  The row is read once,
-// its exponentials are made once and scaled into the gradient.
+// Short rows: G lanes of a wave hold one row in registers (NV pieces of 16 bytes to a lane), 64 / G rows to a wave.  The row is read once.
+// Bound by issue and latency rather than bytes for the smallest: 4.2 M rows of 5 fp32 actions with avail took 108 us at five waves to a SIMD and with the row
+// waiting for its token, 70 us (4.6 TB/s) at eight and without.  65536 rows of 1032 bf16 columns: 101 us; a workgroup per row: 261.
 template <class T, int MODE, bool AV, bool EN, int G, int NV>
 __global__ __launch_bounds__(256, NV * G < 256 ? 8 : NV == 4 ? 5 : 4) void k_tok_short(const TokArgs a) {
     typedef typename T::elem elem;
@@ -468,6 +445,7 @@ __global__ __launch_bounds__(256, NV * G < 256 ? 8 : NV == 4 ? 5 : 4) void k_tok
 }
 
 // Long rows: a workgroup holds a row in registers, NV pieces of 16 bytes to a thread, so that the logits leave memory once.  Workgroups are
+// (8192 x 131072 bf16: 0.81 ms, 5.3 TB/s, where a large copy gets 5.0; reading each row twice took 1.38 ms.)  They are
 // persistent; a piece's register is refilled with the NEXT row as soon as its gradient is stored, so loads are in flight during all of the arithmetic and no second workgroup is needed to hide them.
 // That only works in straight-line code -- behind a branch the compiler waits for every load there is -- so no load depends on a condition:
 // threads without a piece read the row's last one, and where the next row is left out the current one is read again (from a cache).
@@ -656,6 +634,7 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
     // rounds of 4096 columns took 23 us
 #define TOK_SHORT(G, NV) do { const int grid = MODE == TOK_POLICY && a.rows <= (G < 64 ? 4 : 1) * (256 / G) ? 1 : tok_grid((a.rows + 256 / G - 1) / (256 / G)); \
         hipLaunchKernelGGL((k_tok_short<T, MODE, AV, EN, G, NV>), dim3(grid), dim3(256), 0, s, a); return grid; } while (0)
+    // the fewest lanes that hold the row, so that most of a wave works: up to 512 pieces (measured at 130 and 512: the wave is faster than a workgroup)
     if (nvec <= 2) TOK_SHORT(1, 2);
     if (nvec <= 8) TOK_SHORT(4, 2);
     if (nvec <= 32) TOK_SHORT(16, 2);
@@ -665,11 +644,14 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
 #undef TOK_SHORT
     const int64_t nfull = a.V / T::W;
     a.peel = 127u;
-    if constexpr (MODE == TOK_BWD) {
+    auto back = [&](const TokArgs& b) {
         constexpr int NT = 256, U = 4;
         const int parts = (int)((nfull + NT * U - 1) / (NT * U));
-        const int64_t tiles = a.rows * parts;
-        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, a, parts, tiles);
+        const int64_t tiles = b.rows * parts;
+        hipLaunchKernelGGL((k_tok_back<T, AV, EN, NT, U>), dim3((unsigned)(tiles < (1 << 20) ? tiles : (1 << 20))), dim3(NT), 0, s, b, parts, tiles);
+    };
+    if constexpr (MODE == TOK_BWD) {
+        back(a);
         return 0;
     }
     if constexpr (MODE == TOK_LOGP) {
@@ -684,12 +666,13 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
             return 0;
         }
         const int grid = (int)(a.rows < (1 << 20) ? a.rows : (1 << 20));
-        hipLaunchKernelGGL((k_tok_sum<T, AV, EN, 256, 2>), dim3(grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((k_tok_sum<T, MODE, AV, EN, 256, 2>), dim3(grid), dim3(256), 0, s, a);
         return grid;
     }
     if constexpr (MODE == TOK_POLICY) {
         constexpr int HEAD = (128 / (int)sizeof(typename T::elem) + T::W - 1) / T::W;  // the most pieces that a head takes from the body
-        // FULL pieces of every thread exist: nfull > NT * FULL; a head is only peeled off where they still do
+        // The smallest workgroup whose registers hold the row, four pieces to a thread at a time: threads without a piece still load and mask.  FULL pieces of
+        // every thread exist: nfull > NT * FULL; a head is only peeled off where they still do.
 #define TOK_REGS(NT, NV, FULL, PER_CU) do { if (nfull <= NT * NV) { const int grid = (int)(a.rows < 256 * PER_CU ? a.rows : 256 * PER_CU); \
         a.peel = nfull - HEAD >= NT * FULL ? 127u : 0u; \
         hipLaunchKernelGGL((k_tok_regs<T, AV, EN, NT, NV, FULL>), dim3(grid), dim3(NT), 0, s, a); return grid; } } while (0)
@@ -701,13 +684,21 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
         TOK_REGS(512, 16, 12, 2);
         TOK_REGS(1024, 12, 8, 1);
         TOK_REGS(1024, 16, 12, 1);
+        if constexpr (!AV) TOK_REGS(1024, 20, 16, 1);  // (with avail their LDS would not do.)  4096 x 151936 bf16: 0.50 ms, in two launches 0.62
 #undef TOK_REGS
     }
-    if constexpr (MODE == TOK_POLICY) {
+    if constexpr (MODE == TOK_POLICY) {  // three sweeps of memory at 5 TB/s and more instead of two that a workgroup could overlap only by half (3.0 TB/s)
         const int grid = tok_grid(a.rows);
-        hipLaunchKernelGGL((k_tok_stream<T, AV, EN, 256>), dim3(grid), dim3(256), 0, s, a);
+        a.peel = 127u;
+        a.keep = reinterpret_cast<float2*>(scratch);
+        a.g_out = reinterpret_cast<float*>(a.keep + a.rows); a.h_out = a.g_out + a.rows; a.entropy = a.h_out + a.rows;
+        hipLaunchKernelGGL((k_tok_sum<T, MODE, AV, true, 256, 2>), dim3(grid), dim3(256), 0, s, a);
+        TokArgs b = a;
+        b.keep_in = a.keep; b.d_logp = a.g_out; b.d_entropy = a.h_out; b.entropy_in = a.entropy;
+        back(b);
         return grid;
     }
+    return 0;
 }
 template <class T, int MODE>
 int tok_launch2(TokArgs& a, bool en, void* scratch, hipStream_t s) {
