@@ -36,7 +36,7 @@ class MultiAdamW:
     state_bits 32 or 8.  max_norm > 0 clips all gradients by their global norm (``norm[0]`` is the norm of the last step, ``norm[1]`` the
     factor applied).  copies: per parameter a tensor (or None) that receives its new value in another type.  capturable: the step
     counter lives on the device, so that a captured step() counts on at every replay; a captured step reads the gradients
-    at the addresses they had."""
+    at the addresses they had and keeps the learning rate, decay, eps and max_norm it was captured with."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=0.0, copies=None, capturable=False):
         self.params = list(params)
@@ -97,7 +97,7 @@ class MultiAdamW:
 
     def step(self, grads=None, grad_scale=1.0):
         """One step on ``grads`` (per parameter a tensor or None; default: each parameter's .grad).  A parameter without a gradient
-        is left alone, its states too.  Gradients are read, multiplied by grad_scale on the way, never written."""
+        is left alone, its states too; the bias correction counts this optimiser's steps.  Gradients are read, multiplied by grad_scale on the way, never written."""
         params, index = self.params, self.device.index
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != len(params):
@@ -112,10 +112,10 @@ class MultiAdamW:
         shapes, kinds = ([t[i] for i in have] for t in (self._shapes, self._dtypes)) if some else (self._shapes, self._dtypes)
         # the whole list at once (there may be hundreds of tensors); only a list that is not as it should be is looked through
         if not ([p.shape for p in params] == shapes == [g.shape for g in grads] and [p.dtype for p in params] == kinds and all(map(_contiguous, params))
-                and all(map(_contiguous, grads)) and all(g.get_device() == index and g.dtype in _DTYPES for g in grads)):
+                and all(map(_contiguous, grads)) and all(p.get_device() == index for p in params) and all(g.get_device() == index and g.dtype in _DTYPES for g in grads)):
             for i, p, g, shape, kind in zip(have, params, grads, shapes, kinds):
-                if p.shape != shape or p.dtype != kind or not p.is_contiguous():
-                    raise ValueError(f"params[{i}] has another type, shape or layout than at the start")
+                if p.shape != shape or p.dtype != kind or p.device != self.device or not p.is_contiguous():
+                    raise ValueError(f"params[{i}] has another device, type, shape or layout than at the start")
                 _tensor(g, f"grads[{i}]", like=p)
         table = np.zeros(len(have), _ENTRY)
         for name in ("n", "block", "param_dtype", "copy_dtype"):
@@ -124,8 +124,8 @@ class MultiAdamW:
         table["grad"] = list(map(_address, grads))
         table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
         if self._has_copies:
-            if any(c is not None and (c.shape != p.shape or _DTYPES.get(c.dtype) != k or not c.is_contiguous()) for c, p, k in zip(copies, params, fixed["copy_dtype"])):
-                raise ValueError("copies: one has another type, shape or layout than at the start")
+            if any(c is not None and (c.shape != p.shape or c.get_device() != index or _DTYPES.get(c.dtype) != k or not c.is_contiguous()) for c, p, k in zip(copies, params, fixed["copy_dtype"])):
+                raise ValueError("copies: one has another device, type, shape or layout than at the start")
             table["copy"] = [0 if c is None else c.data_ptr() for c in copies]
         lib = N.load()
         with N.on_device(index):
@@ -138,7 +138,10 @@ class MultiAdamW:
                         self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, self.max_norm if clip else 0.0, grad_scale,
                         self.norm.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
                         None if self.step_dev is None else self.step_dev.data_ptr(), self.steps + 1, self.state_bits)
-            N.check(lib.cm_adamw_multi_step(table.ctypes.data, len(have), C.byref(o), N.raw_stream(index)), "cm_adamw_multi_step")
+            rc = lib.cm_adamw_multi_step(table.ctypes.data, len(have), C.byref(o), N.raw_stream(index))
+            if rc and self.capturable:
+                self.step_dev.sub_(1)  # a step that was refused is none
+            N.check(rc, "cm_adamw_multi_step")
         self.steps += 1
 
     def load_state(self, exp_avg, second, scale=None, step=0):

@@ -68,7 +68,7 @@ __device__ __forceinline__ TokSum tok_careful_sum(const typename T::elem* row, c
     tok_block<EN, NT / 64>(z, a.c.bin, sh);
     return z;
 }
-// ... and its gradient, or zeros (g == nullptr)
+// ... and its gradient, or zeros (not live)
 template <class T, bool AV, bool EN, int NT>
 __device__ __forceinline__ void tok_careful_grad(const typename T::elem* row, const uint8_t* av, typename T::elem* drow, const TokArgs& a, const TokGrad& g, bool live) {
     for (int j = threadIdx.x * T::W; j < a.V; j += NT * T::W) {
@@ -173,7 +173,6 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
     if (MODE == TOK_POLICY && tid == 0)
         for (int i = 0; i < TOK_STATS; ++i) { if (gridDim.x == 1) a.stats[i] = (float)st[i]; else a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i]; }
 }
-
 
 // Few long rows: a row is cut into segments, a workgroup sums one, k_tok_join puts them together.  (16 rows of 131072 bf16 columns: 13.3 us with
 // a workgroup per row.)
@@ -444,9 +443,8 @@ __global__ __launch_bounds__(256, NV * G < 256 ? 8 : NV == 4 ? 5 : 4) void k_tok
     }
 }
 
-// Long rows: a workgroup holds a row in registers, NV pieces of 16 bytes to a thread, so that the logits leave memory once.  Workgroups are
-// (8192 x 131072 bf16: 0.81 ms, 5.3 TB/s, where a large copy gets 5.0; reading each row twice took 1.38 ms.)  They are
-// persistent; a piece's register is refilled with the NEXT row as soon as its gradient is stored, so loads are in flight during all of the arithmetic and no second workgroup is needed to hide them.
+// Long rows: a workgroup holds a row in registers, NV pieces of 16 bytes to a thread, so that the logits leave memory once
+// (8192 x 131072 bf16: 0.81 ms, 5.3 TB/s, where a large copy gets 5.0; reading each row twice took 1.38 ms).  Workgroups are persistent; a piece's register is refilled with the NEXT row as soon as its gradient is stored, so loads are in flight during all of the arithmetic and no second workgroup is needed to hide them.
 // That only works in straight-line code -- behind a branch the compiler waits for every load there is -- so no load depends on a condition:
 // threads without a piece read the row's last one, and where the next row is left out the current one is read again (from a cache).
 // The first FULL pieces of every thread exist (the choice of the kernel sees to that).

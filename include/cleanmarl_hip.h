@@ -515,8 +515,8 @@ int cm_polyak_update(float* target, const float* src, int64_t n, double polyak, 
  * actor passes above do behind their MLP (cleanmarl/mappo_multienvs.py:172-183, 536-570).  A row of `vocab` logits is divided by
  * `temperature`; columns with avail == 0 do not take part, whatever the logits hold there (NaN and infinities included), and
  * get a zero gradient.  A row is LEFT OUT -- log-probability, entropy and gradient 0, not counted -- if its token is negative (padding),
- * its weight is 0 or none of its columns is available (every logit -inf counts as that); the logits of a row that is left out for its
- * token or weight are not read.  A token >= vocab gives NaN.  The gradient has the logits' type, is rounded once, and may be
+ * its weight is 0 or none of its columns is available (every logit -inf counts as that); what the logits of such a row hold does
+ * not matter.  A token >= vocab gives NaN.  The gradient has the logits' type, is rounded once, and may be
  * written over the logits (dlogits == logits with the same row stride); any other overlap is refused.  Per-row vectors are fp32 and contiguous.
  * All sums are formed in a fixed order, which may depend on the alignment of the rows: the same inputs at equal alignments give the same bits. */
 enum { CM_DTYPE_F32 = 0, CM_DTYPE_F16 = 1, CM_DTYPE_BF16 = 2 };

@@ -126,6 +126,7 @@ def test_wrapper_refuses_what_it_cannot_step():
 
 @pytest.mark.gpu
 def test_wrapper_refusals_on_the_device():
+    from cleanmarl_amd._native import NativeError
     from cleanmarl_amd.adamw import MultiAdamW
     p = torch.zeros(8, 4).cuda()
     for bad in (dict(params=[p, p]), dict(params=[p, p.view(-1)[4:9]]), dict(params=[p.t()]), dict(params=[p.double()]), dict(params=[p], copies=[]), dict(params=[p], copies=[p]),
@@ -136,6 +137,18 @@ def test_wrapper_refusals_on_the_device():
     for bad in ([], [torch.zeros(4, 8).cuda()], [torch.zeros(8, 4)], [torch.zeros(4, 8).cuda().t()], [torch.zeros(8, 4).cuda().double()]):
         with pytest.raises(ValueError):
             o.step(bad)
+    q, low = torch.zeros(8, 4).cuda(), torch.zeros(8, 4, dtype=torch.bfloat16).cuda()
+    moved = MultiAdamW([q], copies=[low])
+    for t in (q, low):  # a tensor that has left the device since
+        there, t.data = t.data, t.data.cpu()
+        with pytest.raises(ValueError, match="another device"):
+            moved.step([torch.zeros(8, 4).cuda()])
+        t.data = there
+    counted = MultiAdamW([q], capturable=True)
+    counted.betas = (1.0, 0.9)
+    with pytest.raises(NativeError, match="beta1"):
+        counted.step([torch.zeros(8, 4).cuda()])
+    assert counted.state_dict()["step"] == counted.steps == 0
     with pytest.raises(AttributeError):
         o.root_avg_sq
     with pytest.raises(ValueError):

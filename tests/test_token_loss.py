@@ -381,7 +381,7 @@ def _policy_case(x, tok, mask, T, seed, kl=0.1, ent=0.02):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V", [3, 40, 700, 5000, 70000, 140002])
+@pytest.mark.parametrize("V", [3, 40, 700, 5000, 70000, 140002, 170002])
 def test_policy_loss_on_rows_of_every_size(V, dtype):
     """Rows beside each other that are ordinary, far from zero, of one value (the type's lowest), with -inf among them, or all -inf; small temperatures."""
     gen = torch.Generator().manual_seed(V)
@@ -512,7 +512,7 @@ def test_many_rows(rows, V):
 # ---------------------------------------------------------------------------------------------------------------- preference loss
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("lengths, V, front, behind", [([1, 1], 5, 0, 0), ([3, 0, 7, 2], 100, 2, 3), ([40, 1, 300, 17, 5, 90], 1030, 0, 5), ([2, 5, 3, 1], 40000, 1, 0), ([600, 500], 64, 0, 9),
+@pytest.mark.parametrize("lengths, V, front, behind", [([1, 1], 5, 0, 0), ([3, 0, 7, 2], 100, 2, 3), ([40, 1, 300, 17, 5, 90], 1030, 0, 5), ([2, 5, 3, 1], 40000, 1, 0), ([(7 * i) % 5 for i in range(1300)], 12, 1, 2), ([1] * 600, 9000, 0, 1), ([600, 500], 64, 0, 9),
                                                         ([2, 1, 1, 3], 140001, 0, 2)])
 def test_preference_loss(lengths, V, front, behind, dtype):
     from cleanmarl_amd import token_loss as TL
