@@ -353,7 +353,8 @@ def _own(s):
         r = TL.policy_loss_fwd_bwd(s["logits"], s["token"], s["logp_old"], s["adv"], logp_ref=s["logp_ref"], weight=s["weight"], avail=s["mask"],
                                    temperature=s["temperature"], clip_low=CLIP_LOW, clip_high=CLIP_HIGH, kl_coef=s["kl"], entropy_coef=s["entropy"])
         return {"stats": r.stats, "logp": r.logp, "dlogits": r.dlogits}
-    r = TL.preference_loss_fwd_bwd(s["logits"], s["token"], s["seq_start"], s["logp_ref"], beta=BETA, label_smoothing=s["smoothing"], kind=s["kind"],
+    r = TL.preference_loss_fwd_bwd(s["logits"], s["token"], s["seq_start"], s["logp_ref"], beta=BETA, kind=s["kind"],
+                                   label_smoothing=s["smoothing"] if s["kind"] == "sigmoid" else 0.0,  # the squared loss has none and refuses it
                                    scale=1.0 / s["pairs"], out=s["dlogits"])
     return {"stats": r.stats[:6], "margin": r.margin, "seq_logp": r.seq_logp, "dlogits": r.dlogits}
 
