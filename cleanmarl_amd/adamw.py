@@ -17,7 +17,7 @@ _DTYPES = {torch.float32: N.DTYPE_F32, torch.float16: N.DTYPE_F16, torch.bfloat1
 _ENTRY = np.dtype([("param", np.uint64), ("grad", np.uint64), ("copy", np.uint64), ("n", np.int64), ("block", np.int64),
                    ("param_dtype", np.int32), ("grad_dtype", np.int32), ("copy_dtype", np.int32), ("reserved", np.int32)])  # cm_adamw_tensor_t
 
-_contiguous, _address = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+_contiguous, _address, _index, _shape, _type = torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.get_device, torch.Tensor.shape.__get__, torch.Tensor.dtype.__get__
 
 
 def _tensor(t, what, like=None):
@@ -111,8 +111,10 @@ class MultiAdamW:
         fixed = self._fixed[have] if some else self._fixed
         shapes, kinds = ([t[i] for i in have] for t in (self._shapes, self._dtypes)) if some else (self._shapes, self._dtypes)
         # the whole list at once (there may be hundreds of tensors); only a list that is not as it should be is looked through
-        if not ([p.shape for p in params] == shapes == [g.shape for g in grads] and [p.dtype for p in params] == kinds and all(map(_contiguous, params))
-                and all(map(_contiguous, grads)) and all(p.get_device() == index for p in params) and all(g.get_device() == index and g.dtype in _DTYPES for g in grads)):
+        # (228 small tensors: 0.16 ms on the host with a generator for each check, 0.14 with these)
+        types = list(map(_type, grads))
+        if not (list(map(_shape, params)) == shapes == list(map(_shape, grads)) and list(map(_type, params)) == kinds and all(map(_contiguous, params))
+                and all(map(_contiguous, grads)) and {index}.issuperset(map(_index, params)) and {index}.issuperset(map(_index, grads)) and _DTYPES.keys() >= set(types)):
             for i, p, g, shape, kind in zip(have, params, grads, shapes, kinds):
                 if p.shape != shape or p.dtype != kind or p.device != self.device or not p.is_contiguous():
                     raise ValueError(f"params[{i}] has another device, type, shape or layout than at the start")
@@ -122,7 +124,7 @@ class MultiAdamW:
             table[name] = fixed[name]
         table["param"] = list(map(_address, params))
         table["grad"] = list(map(_address, grads))
-        table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
+        table["grad_dtype"] = list(map(_DTYPES.__getitem__, types))
         if self._has_copies:
             if any(c is not None and (c.shape != p.shape or c.get_device() != index or _DTYPES.get(c.dtype) != k or not c.is_contiguous()) for c, p, k in zip(copies, params, fixed["copy_dtype"])):
                 raise ValueError("copies: one has another device, type, shape or layout than at the start")
