@@ -126,9 +126,12 @@ class MultiAdamW:
         table["grad"] = list(map(_address, grads))
         table["grad_dtype"] = list(map(_DTYPES.__getitem__, types))
         if self._has_copies:
-            if any(c is not None and (c.shape != p.shape or c.get_device() != index or _DTYPES.get(c.dtype) != k or not c.is_contiguous()) for c, p, k in zip(copies, params, fixed["copy_dtype"])):
+            at = [i for i, c in enumerate(copies) if c is not None]
+            there = [copies[i] for i in at]
+            if not (list(map(_shape, there)) == [shapes[i] for i in at] and list(map(_DTYPES.get, map(_type, there))) == table["copy_dtype"][at].tolist()
+                    and all(map(_contiguous, there)) and {index}.issuperset(map(_index, there))):
                 raise ValueError("copies: one has another device, type, shape or layout than at the start")
-            table["copy"] = [0 if c is None else c.data_ptr() for c in copies]
+            table["copy"][at] = list(map(_address, there))
         lib = N.load()
         with N.on_device(index):
             clip = self.max_norm is not None and self.max_norm > 0
