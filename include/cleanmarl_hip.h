@@ -556,7 +556,7 @@ int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* logp_old, con
  * ascending, within [0, rows]); sequence i is the chosen and pairs + i the rejected answer of pair i.  L_q = sum of the sequence's
  * log-probabilities (64-bit sums; tokens < 0 -- prompts, padding -- are left out), logp_ref [2 pairs] the reference policy's sums,
  *   margin = (L_i - ref_i) - (L_{P+i} - ref_{P+i}),  z = beta margin
- *   CM_PREFERENCE_SIGMOID: -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing;   CM_PREFERENCE_SQUARED: (margin - 1/(2 beta))^2
+ *   CM_PREFERENCE_SIGMOID: -(1 - e) log sigmoid(z) - e log sigmoid(-z), e = label_smoothing;   CM_PREFERENCE_SQUARED: (margin - 1/(2 beta))^2 (e has to be 0)
  * dlogits = scale * d(sum of losses)/dlogits (scale = 1 / pairs: the mean).  Rows in front of the first and behind the last sequence are
  * not touched.  margin [pairs], seq_logp [2 pairs] may be NULL.  stats[CM_NUM_STATS]: sums over the pairs, slots CM_PREF_*. */
 enum { CM_PREFERENCE_SIGMOID = 0, CM_PREFERENCE_SQUARED = 1 };
