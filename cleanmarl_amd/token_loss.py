@@ -159,8 +159,8 @@ def preference_loss_fwd_bwd(logits, token, seq_start, logp_ref, beta=0.1, label_
 
     ``logits`` [rows, vocab]: the packed rows of 2P sequences, the P chosen answers first, then the P rejected ones; sequence q has the rows
     ``seq_start[q]:seq_start[q + 1]`` (int32, on the device).  Tokens that are not part of an answer are negative.  ``logp_ref`` [2P]: the
-    reference policy's sums.  ``kind``: "sigmoid", or "squared" (without label_smoothing).  ``scale``: factor of the gradient, 1/P (the mean over the pairs) by default.  Rows outside all sequences of
-    ``out`` are not written (zeros in a tensor that is made here)."""
+    reference policy's sums.  ``kind``: "sigmoid", or "squared" (without label_smoothing).  ``scale``: factor of the gradient, 1/P (the mean
+    over the pairs) by default.  Rows outside all sequences of ``out`` are not written (zeros in a tensor that is made here)."""
     rows = _rows(logits, token, avail, temperature)
     if logits.dim() != 2:
         raise ValueError(f"logits: need [rows, vocab], got {tuple(logits.shape)}")
