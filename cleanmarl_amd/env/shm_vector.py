@@ -11,11 +11,11 @@ those of the reference loop, so `collect_episode` returns exactly what `driver.h
 pipe-per-env protocol.
 """
 import os
-from multiprocessing import Pipe, Process, shared_memory
+from multiprocessing import Pipe, shared_memory
 
 import numpy as np
 
-from .vector import EnvWorkerDied, environment, recv_from_worker, send_to_worker  # noqa: F401
+from .vector import EnvWorkerDied, environment, recv_from_worker, send_to_worker, start_worker  # noqa: F401
 
 
 def _worker(conn, factory_args, lo, hi, names, shapes, index_offset=0):
@@ -78,8 +78,7 @@ class ShmVectorEnv:
             if lo == hi:
                 continue
             parent, child = Pipe()
-            p = Process(target=_worker, args=(child, factory_args, lo, hi, names, self.shapes, index_offset), daemon=True)
-            p.start()
+            p = start_worker(_worker, (child, factory_args, lo, hi, names, self.shapes, index_offset))
             child.close()  # see vector.recv_from_worker: a dead worker must surface as an error, not as a hang
             self.conns.append(parent); self.procs.append(p)
 

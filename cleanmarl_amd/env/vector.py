@@ -3,8 +3,37 @@
 ("sample", None) ("close", None); replies are dicts with the reference's keys.  Kept for real (host) envs --
 PettingZoo / SMAClite adapters written against CommonInterface plug in unchanged.  Actions travel as plain
 int lists (the reference pickles a torch tensor per env per step)."""
+import gc
 import importlib
+import threading
 from multiprocessing import Pipe, Process
+
+_STARTING = threading.RLock()
+
+
+def _begin(target, collects, args):
+    gc.freeze()  # what is there belongs to the parent: no collection of this process looks at it
+    if collects:
+        gc.enable()
+    target(*args)
+
+
+def start_worker(target, args):
+    """A daemon process that runs target(*args) and never finalises an object it inherited.
+
+    A process that drives a GPU leaves dropped objects behind that only a garbage collection ends (page-locked tensors, events, graphs); their
+    finalisers call the GPU's runtime, which does not survive a fork: a worker whose collector came across one died of SIGSEGV.  The collector
+    is off from before the fork until the worker has frozen what it inherited."""
+    with _STARTING:  # two threads: the second would take the first one's pause for the caller's choice
+        collects = gc.isenabled()
+        gc.disable()
+        try:
+            p = Process(target=_begin, args=(target, collects, args), daemon=True)
+            p.start()
+        finally:
+            if collects:
+                gc.enable()
+    return p
 
 
 def environment(env_type, env_name, env_family, agent_ids, kwargs=None, index=0, seed=1, synthetic=None):
@@ -93,8 +122,7 @@ class PipeVectorEnv:
         self.conns, self.procs = [], []
         for i in range(n):
             parent, child = Pipe()
-            p = Process(target=env_worker, args=(child, dict(factory_args, index=index_offset + i)), daemon=True)
-            p.start()
+            p = start_worker(env_worker, (child, dict(factory_args, index=index_offset + i)))
             child.close()  # the parent's copy of the child's end: with it open a dead worker never produces an EOFError here
             self.conns.append(parent)
             self.procs.append(p)
