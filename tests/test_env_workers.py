@@ -106,3 +106,41 @@ def test_nothing_inherited_is_finalised_in_a_worker(kind, collecting, monkeypatc
         pids = [int(line) for line in f.read().split()]
     os.close(states); os.close(report)
     assert pids == [os.getpid()] * 20, f"{sum(p != os.getpid() for p in pids)} finalisers ran in workers"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("recurrent", [False, True])
+def test_a_host_rollout_leaves_torchs_host_threads_alone(recurrent):
+    """The env workers need the cores: no step of an episode runs a torch operation between host tensors (one of this size would wake every thread of torch's
+    pool, and they spin)."""
+    import torch
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from cleanmarl_amd.env.shm_vector import ShmVectorEnv
+    from cleanmarl_amd.gru import GRUPPOLearner
+    from cleanmarl_amd.host_rollout import PinnedHostRollout
+    from cleanmarl_amd.learner import HParams, NetSpec, PPOLearner
+
+    class OnTheHost(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            there = [t for t in (*args, out) if isinstance(t, torch.Tensor)]
+            if len(there) > 1 and all(t.device.type == "cpu" for t in there) and max(t.numel() for t in there) > 10000:
+                seen.append(str(func))
+            return out
+
+    seen, E, A, T = [], 64, 8, 6
+    dev = torch.device("cuda:0")
+    fac = dict(env_type="synthetic_cpu", env_name="x", env_family="mpe", agent_ids=True, kwargs={}, seed=3, synthetic=dict(agents=A, steps=T))
+    kind = GRUPPOLearner if recurrent else PPOLearner
+    v = ShmVectorEnv(E, fac, n_workers=2)
+    actor = NetSpec(7 * A, 64, 0, 5, "gru") if recurrent else NetSpec(7 * A, 64, 1, 5)
+    roll = PinnedHostRollout(v, kind("mappo", actor, NetSpec(6 * A * A, 64, 1, 1), A, HParams(), dev), recurrent, dev, t_cap=T)
+    try:
+        assert min(a.size for a in (v.arr["obs"], v.arr["state"])) > 10000  # blocks that count
+        roll.collect(1)
+        with OnTheHost():
+            roll.collect(2)
+    finally:
+        roll.close()
+        v.close()
+    assert seen == []
