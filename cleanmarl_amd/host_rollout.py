@@ -42,11 +42,15 @@ class PinnedHostRollout:
         self.buf = DeviceBatch(self.E, self.A, self.cap, self.Do, self.Ds, self.K, device, pad_obs=self.pad, pad_state=self.pad)
         self.h = None
         self.ws = None
+        self.stream = None
         self.calls = 0
 
     def close(self):
-        """The shared blocks belong to the vector env; lets go of the views of them."""
-        self.shared = None
+        """Lets go of the page-locked twins, once no copy uses them any more, and of the views of the shared blocks, which belong to the vector env."""
+        if self.stream is not None:  # an episode that ended in an error may have left copies behind
+            self.stream.synchronize()
+        self.shared = self.twins = self.stream = None
+        self.h_obs = self.h_state = self.h_avail = self.h_act = None
 
     def _grow(self):
         old, T0 = self.buf, self.cap
@@ -88,7 +92,7 @@ class PinnedHostRollout:
         ep_len = np.zeros(E, np.int64)
         ep_info = [None] * E
         alive = np.arange(E)
-        stream = torch.cuda.current_stream()
+        self.stream = stream = torch.cuda.current_stream()
         t = 0
         while alive.size:
             if t == self.cap:

@@ -108,6 +108,36 @@ def test_nothing_inherited_is_finalised_in_a_worker(kind, collecting, monkeypatc
     assert pids == [os.getpid()] * 20, f"{sum(p != os.getpid() for p in pids)} finalisers ran in workers"
 
 
+def test_a_closed_host_rollout_keeps_no_page_locked_memory(monkeypatch):
+    """Whoever still refers to it (a reference cycle, a frame that a forked worker inherits): close() itself lets go of the twins, behind the copies that use them."""
+    import weakref
+
+    import torch
+    from cleanmarl_amd import host_rollout
+    from cleanmarl_amd.env.shm_vector import ShmVectorEnv
+
+    class Stream:
+        def synchronize(self):
+            order.append(len([w for w in twins if w() is not None]))
+
+    order, real = [], torch.empty
+    monkeypatch.setattr(host_rollout.torch, "empty", lambda *a, pin_memory=False, **kw: real(*a, **kw))  # ordinary memory stands in for page-locked
+    monkeypatch.setattr(host_rollout.N, "load", lambda: None)
+    fac = dict(env_type="synthetic_cpu", env_name="x", env_family="mpe", agent_ids=True, kwargs={}, seed=3, synthetic=dict(agents=2, steps=3))
+    v = ShmVectorEnv(3, fac, n_workers=1)
+    roll = host_rollout.PinnedHostRollout(v, None, False, torch.device("cpu"), t_cap=3)
+    roll.myself = roll
+    try:
+        twins = [weakref.ref(t) for t in (roll.h_obs, roll.h_state, roll.h_avail, roll.h_act)]
+        roll.stream = Stream()
+        roll.close()
+        assert order == [4] and [w() for w in twins] == [None] * 4
+        roll.close()  # closing twice is closing once
+        assert order == [4]
+    finally:
+        v.close()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("recurrent", [False, True])
 def test_a_host_rollout_leaves_torchs_host_threads_alone(recurrent):
