@@ -33,7 +33,7 @@ def _tensor(t, what, like=None):
 class MultiAdamW:
     """params: tensors of one GPU, each float32, float16 or bfloat16 and contiguous, no two sharing memory.
 
-    state_bits 32 or 8.  max_norm > 0 clips all gradients by their global norm (``norm[0]`` is the norm of the last step, ``norm[1]`` the
+    state_bits 32 or 8 (a NaN code in root_avg_sq stands for infinity: an element whose second moment has left fp32).  max_norm > 0 clips all gradients by their global norm (``norm[0]`` is the norm of the last step, ``norm[1]`` the
     factor applied).  copies: per parameter a tensor (or None) that receives its new value in another type.  capturable: the step
     counter lives on the device, so that a captured step() counts on at every replay; a captured step reads the gradients
     at the addresses they had and keeps the learning rate, decay, eps and max_norm it was captured with."""

@@ -10,7 +10,8 @@
 // two tensors and an arena is one allocation to checkpoint.  With 8 bits a block keeps m and sqrt v as e4m3 codes times a scale that maps
 // its largest magnitude to 448.  sqrt v and not v: the code's 2^-9 .. 448 then spans 11 decades of v.  A sqrt v above zero keeps at least
 // the smallest code: rounded to zero it would leave eps alone under a moment m that was not.  The update itself uses the new moments
-// before they are rounded.
+// before they are rounded.  An element whose moments have left fp32 has no part in its block's scales: sqrt v is a NaN code, read as infinity
+// (its steps are 0 from then on, as with 32 bits, or NaN if m is none that is finite), m a zero or a NaN code.
 #include "cm_common.h"
 #include <float.h>
 #include <math.h>
@@ -162,6 +163,8 @@ __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a
                 m[4 * q] = m0[0] * sm; m[4 * q + 1] = m0[1] * sm; m[4 * q + 2] = m1[0] * sm; m[4 * q + 3] = m1[1] * sm;
                 r[4 * q] = r0[0] * sr; r[4 * q + 1] = r0[1] * sr; r[4 * q + 2] = r1[0] * sr; r[4 * q + 3] = r1[1] * sr;
             }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) r[q] = fminf(r[q], INFINITY);  // NaN is infinity, numbers stay
         }
         float tm = 0.0f, tr = 0.0f;
 #pragma unroll
@@ -182,6 +185,16 @@ __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a
         } else {
             const float f = 1.0f / 448.0f, least = 7.888609052210118e-31f;  // 2^-100: below it a scale would lose bits, and what it scales is nothing
             tm = aw_block_max(tm); tr = aw_block_max(tr);
+            if (!(tm < INFINITY && tr < INFINITY)) {  // rare, and the same for all lanes of the block
+                tm = tr = 0.0f;
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const bool finite = fabsf(m[q]) < INFINITY;
+                    if (!(finite && r[q] < INFINITY)) { m[q] = finite ? 0.0f : NAN; r[q] = NAN; }
+                    tm = fmaxf(tm, fabsf(m[q])); tr = fmaxf(tr, r[q]);
+                }
+                tm = aw_block_max(tm); tr = aw_block_max(tr);
+            }
             sm = tm < least ? 0.0f : tm * f; sr = tr < least ? 0.0f : tr * f;
             const float bm = sm > 0.0f ? 1.0f / sm : 0.0f, br = sr > 0.0f ? 1.0f / sr : 0.0f;
 #pragma unroll

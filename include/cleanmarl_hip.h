@@ -571,6 +571,8 @@ int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* seq_start, in
  * blocks [t.block, t.block + cm_adamw_state_blocks(t.n)); entries come in ascending block order and do not share blocks.  Arenas are
  * zeroed once by the caller, 16-byte aligned, and keep zeros behind a tensor's last element.
  *   state_bits 32: exp_avg, exp_avg_sq are fp32.   8: e4m3 codes (OCP, torch.float8_e4m3fn) of m and of sqrt(v), times scale[block][0] / [1].
+ *                  A scale is always finite: an element whose m or v is not has a NaN code of sqrt(v) (read as infinity, as fp32 states would hold it),
+ *                  a zero or NaN code of m, and no part in its block's scales.
  * max_norm > 0 clips the gradients of ALL entries by their global L2 norm (64-bit sum; after grad_scale); out_norm[0] receives the norm, [1] the coefficient.
  * copy (may be NULL) receives the new parameter in copy_dtype.  Tensors are contiguous and aligned to their element.
  * step_dev (device, may be NULL) replaces step for launches that a graph replays: the caller increments it on the stream. */

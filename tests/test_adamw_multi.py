@@ -417,3 +417,33 @@ def test_a_training_run_of_a_token_policy(bits):
         before = [p.detach().clone() for p in params]
         opt.step([p.grad for p in params])
         assert all(bool(torch.isfinite(p).all()) and not torch.equal(p.detach(), q) for p, q in zip(params, before))
+
+
+# ---------------------------------------------------------------------------------------------------------------- values that leave fp32
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan, 1e22, -3e38])
+def test_an_overflow_stays_with_its_element(value):
+    """8-bit states: the elements beside one whose moments are not finite (with 1e22 only the second: 1e22^2 / 1000 is beyond fp32) do what they do beside a
+    zero gradient, bit for bit, and the element itself does what it does with 32-bit states.  512 elements share the first two blocks; 300 is in the second."""
+    from cleanmarl_amd.adamw import MultiAdamW
+    n, at = 700, 300
+    start = tensors([n], [torch.float32], 1)[0]
+    grads = [tensors([n], [torch.float32], 10 + k)[0] for k in range(4)]
+    runs = {}
+    for name, bits, there in (("8", 8, value), ("beside a zero", 8, 0.0), ("32", 32, value)):
+        opt = MultiAdamW([start.clone()], state_bits=bits, lr=1e-2, betas=(0.9, 0.999), weight_decay=0.1)
+        steps = []
+        for k, g in enumerate(grads):
+            g = g.clone()
+            g[at] = there if k == 1 else 0.0  # an ordinary step, the value, two more steps
+            opt.step([g])
+            steps.append(opt.params[0].clone())
+        runs[name] = steps
+        if name == "8":
+            assert bool(torch.isfinite(opt.scale).all())
+    others = torch.arange(n, device="cuda") != at
+    for got, beside, wide in zip(runs["8"], runs["beside a zero"], runs["32"]):
+        assert bool(torch.isfinite(got[others]).all())
+        assert torch.equal(got[others], beside[others])
+        assert torch.equal(got[at], wide[at]) or (bool(got[at].isnan()) and bool(wide[at].isnan())), (got[at].item(), wide[at].item())
+    assert bool(torch.isfinite(runs["8"][-1][at])) == (abs(value) == 1e22 or abs(value) == 3e38)
