@@ -36,7 +36,10 @@ class MultiAdamW:
     state_bits 32 or 8 (a NaN code in root_avg_sq stands for infinity: an element whose second moment has left fp32).  max_norm > 0 clips all gradients by their global norm (``norm[0]`` is the norm of the last step, ``norm[1]`` the
     factor applied).  copies: per parameter a tensor (or None) that receives its new value in another type.  capturable: the step
     counter lives on the device, so that a captured step() counts on at every replay; a captured step reads the gradients
-    at the addresses they had and keeps the learning rate, decay, eps and max_norm it was captured with."""
+    at the addresses they had and keeps the learning rate, decay, eps and max_norm it was captured with.
+
+    A step counts as an in-place operation on the parameters and copies it writes: a backward pass that needs one of them as it was before raises
+    (a replayed graph's steps go uncounted, as those of torch's operations do)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, max_norm=0.0, copies=None, capturable=False):
         self.params = list(params)
@@ -147,6 +150,9 @@ class MultiAdamW:
             if rc and self.capturable:
                 self.step_dev.sub_(1)  # a step that was refused is none
             N.check(rc, "cm_adamw_multi_step")
+        torch.autograd.graph.increment_version(params)  # written behind torch's back: a graph that saved one of them has to notice
+        if self._has_copies:
+            torch.autograd.graph.increment_version(there)
         self.steps += 1
 
     def load_state(self, exp_avg, second, scale=None, step=0):

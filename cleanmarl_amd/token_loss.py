@@ -3,7 +3,8 @@
 The learners of this package train networks whose logits never leave the fused kernels (<= 64 actions).  A policy that is the caller's own
 model hands its logits over instead: ``[..., vocab]`` of any float type, thousands of columns.  Each ``*_fwd_bwd`` call returns the
 statistics AND the gradient of the logits (cleanmarl/mappo_multienvs.py:527-582 on tokens), which goes into the model with
-``logits.backward(result.dlogits)``.  Everything runs on the current HIP stream of the logits' device; nothing synchronises.
+``logits.backward(result.dlogits)``.  ``out=`` over the logits counts as an in-place operation on them: a model whose last
+operation saved its output for its backward pass (tanh, a softmax) raises then.  Everything runs on the current HIP stream of the logits' device; nothing synchronises.
 
 Rows with a negative token (padding), weight 0 or no available column are left out: log-probability, entropy and gradient 0, not counted.
 """
@@ -91,6 +92,13 @@ def _grad(out, logits):
     return out, _row_stride(out, "out")
 
 
+def _wrote(out, given):
+    """The gradient is in `out`; where that is the caller's (`given`), a graph that saved it -- it may lie over the logits -- has to notice."""
+    if given is not None:
+        torch.autograd.graph.increment_version(given)
+    return out
+
+
 def _workspace(nbytes, device):
     return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
 
@@ -126,9 +134,9 @@ def token_logprob_bwd(logits, token, forward, d_logp, d_entropy=None, avail=None
     H = _vector(forward.entropy, token, "forward.entropy") if d_entropy is not None else None
     lib, index = N.load(), logits.get_device()
     with N.on_device(index):
-        out, ld = _grad(out, logits)
-        N.check(lib.cm_token_logprob_bwd(C.byref(rows), forward.keep.data_ptr(), H, dl, dh, out.data_ptr(), ld, N.raw_stream(index)), "cm_token_logprob_bwd")
-    return out
+        d, ld = _grad(out, logits)
+        N.check(lib.cm_token_logprob_bwd(C.byref(rows), forward.keep.data_ptr(), H, dl, dh, d.data_ptr(), ld, N.raw_stream(index)), "cm_token_logprob_bwd")
+    return _wrote(d, out)
 
 
 def policy_loss_fwd_bwd(logits, token, logp_old, adv, logp_ref=None, weight=None, avail=None, temperature=1.0, clip_low=0.2, clip_high=0.2,
@@ -143,14 +151,14 @@ def policy_loss_fwd_bwd(logits, token, logp_old, adv, logp_ref=None, weight=None
     ref, w = _vector(logp_ref, token, "logp_ref"), _vector(weight, token, "weight")
     lib, device, index = N.load(), logits.device, logits.get_device()
     with N.on_device(index):
-        out, ld = _grad(out, logits)
+        d, ld = _grad(out, logits)
         stats = torch.empty(N.NUM_STATS, dtype=torch.float32, device=device)
         logp = torch.empty_like(logp_old)
         nbytes = lib.cm_token_workspace_bytes(rows.rows, rows.vocab)
         ws = _workspace(nbytes, device)
-        N.check(lib.cm_token_policy_fwd_bwd(C.byref(rows), old, ad, ref, w, clip_low, clip_high, kl_coef, entropy_coef, out.data_ptr(), ld, logp.data_ptr(),
+        N.check(lib.cm_token_policy_fwd_bwd(C.byref(rows), old, ad, ref, w, clip_low, clip_high, kl_coef, entropy_coef, d.data_ptr(), ld, logp.data_ptr(),
                                             stats.data_ptr(), ws.data_ptr(), nbytes, N.raw_stream(index)), "cm_token_policy_fwd_bwd")
-    return PolicyLoss(stats, out, logp)
+    return PolicyLoss(stats, _wrote(d, out), logp)
 
 
 def preference_loss_fwd_bwd(logits, token, seq_start, logp_ref, beta=0.1, label_smoothing=0.0, kind="sigmoid", scale=None, avail=None,
@@ -174,15 +182,13 @@ def preference_loss_fwd_bwd(logits, token, seq_start, logp_ref, beta=0.1, label_
         raise ValueError(f"logp_ref: need float32 [{2 * pairs}] on {logits.device}, got {logp_ref.dtype} {tuple(logp_ref.shape)} on {logp_ref.device}")
     lib, device, index = N.load(), logits.device, logits.get_device()
     with N.on_device(index):
-        if out is None:
-            out = torch.zeros_like(logits, memory_format=torch.contiguous_format)
-        out, ld = _grad(out, logits)
+        d, ld = _grad(torch.zeros_like(logits, memory_format=torch.contiguous_format) if out is None else out, logits)
         stats = torch.empty(N.NUM_STATS, dtype=torch.float32, device=device)
         margin = torch.empty(pairs, dtype=torch.float32, device=device)
         seq_logp = torch.empty(2 * pairs, dtype=torch.float32, device=device)
         nbytes = lib.cm_preference_workspace_bytes(rows.rows, rows.vocab, pairs)
         ws = _workspace(nbytes, device)
         N.check(lib.cm_preference_fwd_bwd(C.byref(rows), seq_start.data_ptr(), pairs, logp_ref.data_ptr(), beta, label_smoothing, _KINDS[kind],
-                                          1.0 / pairs if scale is None else scale, out.data_ptr(), ld, margin.data_ptr(), seq_logp.data_ptr(),
+                                          1.0 / pairs if scale is None else scale, d.data_ptr(), ld, margin.data_ptr(), seq_logp.data_ptr(),
                                           stats.data_ptr(), ws.data_ptr(), nbytes, N.raw_stream(index)), "cm_preference_fwd_bwd")
-    return PreferenceLoss(stats, out, margin, seq_logp)
+    return PreferenceLoss(stats, _wrote(d, out), margin, seq_logp)

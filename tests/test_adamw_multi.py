@@ -447,3 +447,29 @@ def test_an_overflow_stays_with_its_element(value):
         assert torch.equal(got[others], beside[others])
         assert torch.equal(got[at], wide[at]) or (bool(got[at].isnan()) and bool(wide[at].isnan())), (got[at].item(), wide[at].item())
     assert bool(torch.isfinite(runs["8"][-1][at])) == (abs(value) == 1e22 or abs(value) == 3e38)
+
+
+# ---------------------------------------------------------------------------------------------------------------- autograd
+@pytest.mark.gpu
+def test_a_step_is_seen_by_graphs_that_saved_a_parameter():
+    """As with torch's own in-place operations: a backward pass that needs a parameter or a copy as it was before the step says so."""
+    from cleanmarl_amd.adamw import MultiAdamW
+    p = torch.ones(8, 4, device="cuda").requires_grad_(True)
+    low = torch.ones(8, 4, device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    other = torch.ones(3, device="cuda")
+    opt = MultiAdamW([p, other], copies=[low, None])
+    x = torch.ones(4, 8, device="cuda", requires_grad=True)
+    for saved in (x @ p, x.to(torch.bfloat16) @ low):
+        opt.step([torch.ones_like(p.detach()), None])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.sum().backward()
+    versions = [t._version for t in (p, low, other)]
+    opt.step([None, torch.ones(3, device="cuda")])
+    assert [t._version - v for t, v in zip((p, low, other), versions)] == [0, 0, 1]  # what was not written is as it was
+    (x @ p).sum().backward()
+    assert bool(torch.isfinite(x.grad).all())
+    with torch.inference_mode():
+        frozen = torch.ones(4, device="cuda")
+    o = MultiAdamW([frozen, torch.ones(4, device="cuda")])  # tensors made in inference mode count no versions
+    o.step([torch.ones(4, device="cuda")] * 2)
+    assert o.steps == 1 and bool((frozen < 1).all())

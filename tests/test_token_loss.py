@@ -622,3 +622,40 @@ def test_calls_on_two_streams_and_in_graphs():
             calls[(i + 1) % len(calls)]()
             torch.cuda.synchronize()
             assert same(outs[i], want[i]), (k, i)
+
+
+# ---------------------------------------------------------------------------------------------------------------- autograd
+@pytest.mark.gpu
+def test_gradients_over_the_logits_are_seen_by_graphs_that_saved_them():
+    """``out=`` over the logits: a graph whose last operation saved its output (tanh) can no longer run backward and says so; one that did not (a product) can."""
+    from cleanmarl_amd import token_loss as TL
+    rows, V = 4, 40
+    gen = torch.Generator().manual_seed(1)
+    z = torch.randn(rows, V, generator=gen).cuda().requires_grad_(True)
+    w = torch.eye(V).cuda()
+    tok, row = torch.arange(rows).cuda(), torch.full((rows,), -2.0).cuda()
+    seq = torch.tensor([0, 2, 4], dtype=torch.int32).cuda()
+
+    def scored(logits, out):
+        f = TL.token_logprob(logits, tok, keep=True)
+        return TL.token_logprob_bwd(logits, tok, f, row, out=out)
+
+    for call in (scored, lambda logits, out: TL.policy_loss_fwd_bwd(logits, tok, row, row, out=out).dlogits,
+                 lambda logits, out: TL.preference_loss_fwd_bwd(logits, tok, seq, torch.zeros(2).cuda(), out=out).dlogits):
+        logits = torch.tanh(z)
+        d = call(logits.detach(), logits.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            logits.backward(d)
+        logits = torch.tanh(z)
+        before = logits._version
+        d = call(logits.detach(), None)
+        assert logits._version == before
+        want, = torch.autograd.grad(logits, z, d)
+        assert torch.allclose(want, d * (1 - torch.tanh(z).detach() ** 2), rtol=1e-5, atol=1e-7)
+        logits = z @ w
+        d = call(logits.detach(), logits.detach())
+        got, = torch.autograd.grad(logits, z, d.clone())
+        assert torch.equal(got, d)  # (w is the unit matrix)
+    with torch.inference_mode():
+        frozen = torch.zeros(rows, V, device="cuda")
+    assert TL.policy_loss_fwd_bwd(frozen, tok, row, row, out=frozen).dlogits is frozen  # tensors made in inference mode count no versions
