@@ -99,10 +99,14 @@ class MultiAdamW:
         return self._v
 
     def step(self, grads=None, grad_scale=1.0):
-        """One step on ``grads`` (per parameter a tensor or None; default: each parameter's .grad).  A parameter without a gradient
-        is left alone, its states too; the bias correction counts this optimiser's steps.  Gradients are read, multiplied by grad_scale on the way, never written."""
+        """One step on ``grads`` (per parameter a tensor or None; default: each parameter's .grad, of which there has to be one).  A parameter without a
+        gradient is left alone, its states too; the bias correction counts this optimiser's steps.  Gradients are read, multiplied by grad_scale on the way, never written."""
         params, index = self.params, self.device.index
-        grads = [p.grad for p in params] if grads is None else list(grads)
+        if grads is None:
+            grads = [p.grad for p in params]
+            if all(g is None for g in grads):
+                raise ValueError("no parameter has a gradient: a tensor detached from a parameter (p.data) never gets one; hand over the parameters themselves, or grads")
+        grads = list(grads)
         if len(grads) != len(params):
             raise ValueError(f"grads: {len(grads)} for {len(params)} params")
         have = [i for i, g in enumerate(grads) if g is not None]

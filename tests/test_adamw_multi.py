@@ -473,3 +473,28 @@ def test_a_step_is_seen_by_graphs_that_saved_a_parameter():
     o = MultiAdamW([frozen, torch.ones(4, device="cuda")])  # tensors made in inference mode count no versions
     o.step([torch.ones(4, device="cuda")] * 2)
     assert o.steps == 1 and bool((frozen < 1).all())
+
+
+def test_a_step_without_any_gradient_is_an_error():
+    """The default gradients are the parameters' own; where none has one (tensors detached from the parameters never do) nothing would be trained."""
+    from cleanmarl_amd.adamw import MultiAdamW
+    opt = MultiAdamW.__new__(MultiAdamW)  # (the constructor needs a GPU, the refusal does not)
+    opt.params, opt.device, opt.steps = [torch.zeros(3), torch.zeros(4)], torch.device("cuda:0"), 5
+    with pytest.raises(ValueError, match="no parameter has a gradient"):
+        opt.step()
+    assert opt.steps == 5
+
+
+@pytest.mark.gpu
+def test_steps_from_the_parameters_own_gradients():
+    from cleanmarl_amd.adamw import MultiAdamW
+    p, q = (torch.ones(5, device="cuda").requires_grad_(True) for _ in range(2))
+    opt = MultiAdamW([p, q], capturable=True)
+    with pytest.raises(ValueError, match="no parameter has a gradient"):
+        opt.step()
+    assert opt.steps == 0 and opt.step_dev.item() == 0
+    p.sum().backward()
+    opt.step()  # one of them has one
+    assert opt.steps == 1 and bool((p < 1).all()) and bool((q == 1).all())
+    opt.step([None, None])  # said so by the caller
+    assert opt.steps == 2
