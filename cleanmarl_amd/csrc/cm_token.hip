@@ -7,6 +7,7 @@
 // H = log s - sum p_j (x_j - m)  and every gradient below is  dx_j = (g ([j = token] - p_j) + h p_j (log p_j + H)) / T  with two
 // scalars g and h per row.  All sums, statistics and scalars are fp32 or wider; the gradient is rounded once, to the logits' type.
 #include "cm_token.h"
+#include <initializer_list>
 
 namespace {
 
@@ -99,6 +100,25 @@ int tok_check_grad(const char* who, const cm_token_rows_t* t, const void* dlogit
     CM_REQUIRE(same || x + nx <= d || d + nd <= x, "%s: dlogits overlaps the logits without being the same rows", who);
     return 0;
 }
+// What a call writes lies over nothing it reads and over nothing else it writes: rows are read ahead of those that are written, per-row inputs through the scalar
+// cache, which does not see this launch's stores.  (dlogits and logits: tok_check_grad.)  NULL: not there.
+struct TokSpan { const char* name; const void* p; size_t n; };
+int tok_check_apart(const char* who, std::initializer_list<TokSpan> out, std::initializer_list<TokSpan> in) {
+    auto over = [](const TokSpan& a, const TokSpan& b) {
+        const char *x = (const char*)a.p, *y = (const char*)b.p;
+        return x && y && a.n && b.n && x < y + b.n && y < x + a.n;
+    };
+    for (const TokSpan* a = out.begin(); a != out.end(); ++a) {
+        for (const TokSpan* b = out.begin(); b != a; ++b) CM_REQUIRE(!over(*a, *b), "%s: %s overlaps %s", who, a->name, b->name);
+        for (const TokSpan& b : in) CM_REQUIRE(!over(*a, b), "%s: %s overlaps %s", who, a->name, b.name);
+    }
+    return 0;
+}
+size_t tok_bytes(int64_t rows, int64_t ld, int vocab, size_t elem) { return rows > 0 ? ((size_t)(rows - 1) * ld + vocab) * elem : 0; }
+TokSpan tok_span_logits(const cm_token_rows_t* t) { return {"logits", t->logits, tok_bytes(t->rows, t->ld, t->vocab, tok_elem(t->dtype))}; }
+TokSpan tok_span_avail(const cm_token_rows_t* t) { return {"avail", t->avail, tok_bytes(t->rows, t->avail_ld, t->vocab, 1)}; }
+TokSpan tok_span_token(const cm_token_rows_t* t) { return {"token", t->token, (size_t)t->rows * t->token_bytes}; }
+TokSpan tok_span_grad(const cm_token_rows_t* t, const void* d, int64_t ld) { return {"dlogits", d, tok_bytes(t->rows, ld, t->vocab, tok_elem(t->dtype))}; }
 TokArgs tok_args(const cm_token_rows_t* t) {
     TokArgs a = {};
     a.logits = t->logits; a.ld = t->ld; a.avail = t->avail; a.avail_ld = t->avail_ld; a.token = t->token; a.token_bytes = t->token_bytes;
@@ -124,6 +144,9 @@ extern "C" int cm_token_logprob(const cm_token_rows_t* t, float* logp, float* en
     CM_REQUIRE(reinterpret_cast<uintptr_t>(keep) % 8 == 0, "cm_token_logprob: keep must be 8-byte aligned");
     const size_t need = cm_token_workspace_bytes(t->rows, t->vocab);
     CM_REQUIRE(ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "cm_token_logprob: workspace too small (%zu < %zu) or not 16-byte aligned", ws_bytes, need);
+    const size_t row = (size_t)t->rows * sizeof(float);
+    if (int rc = tok_check_apart("cm_token_logprob", {{"logp", logp, row}, {"entropy", entropy, row}, {"keep", keep, 2 * row}, {"the workspace", ws, need}},
+                                 {tok_span_logits(t), tok_span_avail(t), tok_span_token(t)})) return rc;
     TokArgs a = tok_args(t);
     a.logp = logp; a.entropy = entropy; a.keep = (float2*)keep;
     tok_launch(a, t->dtype, TOK_LOGP, entropy != nullptr, ws, (hipStream_t)stream);
@@ -138,6 +161,9 @@ extern "C" int cm_token_logprob_bwd(const cm_token_rows_t* t, const float* keep,
     CM_REQUIRE(t->rows == 0 || (keep && d_logp), "cm_token_logprob_bwd: NULL keep / d_logp");
     CM_REQUIRE(!d_entropy || entropy, "cm_token_logprob_bwd: d_entropy needs the entropy of the forward call");
     CM_REQUIRE(reinterpret_cast<uintptr_t>(keep) % 8 == 0, "cm_token_logprob_bwd: keep must be 8-byte aligned");
+    const size_t row = (size_t)t->rows * sizeof(float);
+    if (int rc = tok_check_apart("cm_token_logprob_bwd", {tok_span_grad(t, dlogits, dlogits_ld)},
+                                 {tok_span_avail(t), tok_span_token(t), {"keep", keep, 2 * row}, {"entropy", entropy, row}, {"d_logp", d_logp, row}, {"d_entropy", d_entropy, row}})) return rc;
     TokArgs a = tok_args(t);
     a.keep_in = (const float2*)keep; a.entropy_in = entropy; a.d_logp = d_logp; a.d_entropy = d_entropy; a.dlogits = dlogits; a.dld = dlogits_ld;
     tok_launch(a, t->dtype, TOK_BWD, d_entropy != nullptr, nullptr, (hipStream_t)stream);
@@ -156,6 +182,11 @@ extern "C" int cm_token_policy_fwd_bwd(const cm_token_rows_t* t, const float* lo
     CM_REQUIRE(kl_coef == 0.0 || logp_ref, "cm_token_policy_fwd_bwd: kl_coef without logp_ref");
     const size_t need = cm_token_workspace_bytes(t->rows, t->vocab);
     CM_REQUIRE(ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "cm_token_policy_fwd_bwd: workspace too small (%zu < %zu) or not 16-byte aligned", ws_bytes, need);
+    const size_t row = (size_t)t->rows * sizeof(float);
+    const TokSpan sums[] = {{"logp", logp, row}, {"stats", stats, CM_NUM_STATS * sizeof(float)}, {"the workspace", ws, need}};
+    if (int rc = tok_check_apart("cm_token_policy_fwd_bwd", {tok_span_grad(t, dlogits, dlogits_ld), sums[0], sums[1], sums[2]},
+                                 {tok_span_avail(t), tok_span_token(t), {"logp_old", logp_old, row}, {"adv", adv, row}, {"logp_ref", logp_ref, row}, {"weight", weight, row}})) return rc;
+    if (int rc = tok_check_apart("cm_token_policy_fwd_bwd", {sums[0], sums[1], sums[2]}, {tok_span_logits(t)})) return rc;
     TokArgs a = tok_args(t);
     a.logp_old = logp_old; a.adv = adv; a.logp_ref = logp_ref; a.weight = weight;
     a.lo = (float)(1.0 - clip_low); a.hi = (float)(1.0 + clip_high); a.kl_coef = (float)kl_coef; a.ent_coef = (float)entropy_coef;
@@ -190,6 +221,11 @@ extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* se
     CM_REQUIRE(kind == CM_PREFERENCE_SIGMOID || label_smoothing == 0.0, "cm_preference_fwd_bwd: the squared loss takes no label_smoothing");
     const size_t need = cm_preference_workspace_bytes(t->rows, t->vocab, pairs);
     CM_REQUIRE(ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(ws) % 16 == 0, "cm_preference_fwd_bwd: workspace too small (%zu < %zu) or not 16-byte aligned", ws_bytes, need);
+    const size_t per_pair = (size_t)pairs * sizeof(float);
+    const TokSpan sums[] = {{"margin", margin, per_pair}, {"seq_logp", seq_logp, 2 * per_pair}, {"stats", stats, CM_NUM_STATS * sizeof(float)}, {"the workspace", ws, need}};
+    if (int rc = tok_check_apart("cm_preference_fwd_bwd", {tok_span_grad(t, dlogits, dlogits_ld), sums[0], sums[1], sums[2], sums[3]},
+                                 {tok_span_avail(t), tok_span_token(t), {"seq_start", seq_start, (2 * (size_t)pairs + 1) * sizeof(int32_t)}, {"logp_ref", logp_ref, 2 * per_pair}})) return rc;
+    if (int rc = tok_check_apart("cm_preference_fwd_bwd", {sums[0], sums[1], sums[2], sums[3]}, {tok_span_logits(t)})) return rc;
     char* w = (char*)ws;
     float2* keep = (float2*)w; w += tok_up((size_t)t->rows * sizeof(float2));
     double* logp = (double*)w; w += tok_up((size_t)t->rows * sizeof(double));

@@ -517,7 +517,8 @@ int cm_polyak_update(float* target, const float* src, int64_t n, double polyak, 
  * get a zero gradient.  A row is LEFT OUT -- log-probability, entropy and gradient 0, not counted -- if its token is negative (padding),
  * its weight is 0 or none of its columns is available (every logit -inf counts as that); what the logits of such a row hold does
  * not matter.  A token >= vocab gives NaN.  The gradient has the logits' type, is rounded once, and may be
- * written over the logits (dlogits == logits with the same row stride); any other overlap is refused.  Per-row vectors are fp32 and contiguous.
+ * written over the logits (dlogits == logits with the same row stride); any other overlap of what a call writes (its workspace, too) with what it
+ * reads or else writes is refused.  Per-row vectors are fp32 and contiguous.
  * All sums are formed in a fixed order, which may depend on the alignment of the rows: the same inputs at equal alignments give the same bits. */
 enum { CM_DTYPE_F32 = 0, CM_DTYPE_F16 = 1, CM_DTYPE_BF16 = 2 };
 typedef struct cm_token_rows {

@@ -659,3 +659,70 @@ def test_gradients_over_the_logits_are_seen_by_graphs_that_saved_them():
     with torch.inference_mode():
         frozen = torch.zeros(rows, V, device="cuda")
     assert TL.policy_loss_fwd_bwd(frozen, tok, row, row, out=frozen).dlogits is frozen  # tensors made in inference mode count no versions
+
+
+# ---------------------------------------------------------------------------------------------------------------- calls that read or write where they must not
+def test_outputs_over_inputs_are_refused():
+    """The policy loss reads its per-row inputs through the scalar cache and ahead of the rows it writes: an output that lies over one of them (the same place, a part of it,
+    or from the other side) is refused; directly in front or behind is not an overlap (then the next refusal is met)."""
+    from cleanmarl_amd import _native as N
+    lib, big = N.load(), 1 << 30
+    t = _rows(avail=0xa0000, avail_ld=8, rows=16)  # 16 rows: 64 bytes of a per-row value, 128 of avail, 512 of logits
+    place = dict(old=0x20000, adv=0x21000, ref=0x22000, w=0x23000, logp=0x24000, stats=0x25000, dx=0x30000, ws=0x40000)
+
+    def call(tt=t, clip_low=0.2, **kw):
+        a = {**place, **kw}
+        rc = lib.cm_token_policy_fwd_bwd(C.byref(tt), a["old"], a["adv"], a["ref"], a["w"], clip_low, 0.2, 0.0, 0.0, a["dx"], 8, a["logp"], a["stats"], a["ws"], big, None)
+        assert rc != 0
+        return lib.cm_last_error().decode()
+
+    for name in ("old", "adv", "ref", "w"):
+        for shift in (0, 60, -60):
+            assert "logp overlaps" in call(logp=place[name] + shift), (name, shift)
+        for shift in (0, 60, -28):
+            assert "stats overlaps" in call(stats=place[name] + shift), (name, shift)
+        for shift in (0, 60, -508):
+            assert "dlogits overlaps" in call(dx=place[name] + shift), (name, shift)
+    assert "logp overlaps" in call(logp=t.token) and "stats overlaps" in call(stats=t.token + 60) and "dlogits overlaps" in call(dx=t.token - 508)
+    assert "logp overlaps" in call(logp=t.logits + 508) and "stats overlaps" in call(stats=t.avail + 124) and "dlogits overlaps" in call(dx=t.avail - 508)
+    assert "logp overlaps" in call(logp=place["dx"] + 4) and "stats overlaps" in call(stats=place["logp"] + 60) and "stats overlaps" in call(stats=place["dx"] + 508)
+    # the other calls
+    p, err = 0x900000, lambda rc: lib.cm_last_error().decode() if rc == -1 else f"rc={rc}"  # noqa: E731
+    for lp, H, keep, ws, text in ((t.logits, None, None, p, "logp overlaps"), (p, p + 60, None, p + 256, "entropy overlaps"), (p, None, t.avail, p + 256, "keep overlaps"),
+                                  (p, None, None, t.token, "the workspace overlaps")):
+        assert text in err(lib.cm_token_logprob(C.byref(t), lp, H, keep, ws, big, None))
+    bwd = dict(keep=0x20000, H=0x21000, dl=0x22000, dh=0x23000)
+    for at in (*bwd.values(), t.token, t.avail):
+        assert "dlogits overlaps" in err(lib.cm_token_logprob_bwd(C.byref(t), *bwd.values(), at - 508, 8, None))
+    pref = dict(seq=0x20000, ref=0x21000, dx=0x30000, margin=0x24000, sums=0x25000, stats=0x26000, ws=0x400000)
+
+    def pairs(**kw):
+        a = {**pref, **kw}
+        return err(lib.cm_preference_fwd_bwd(C.byref(t), a["seq"], 2, a["ref"], 0.1, 0.0, 0, 1.0, a["dx"], 8, a["margin"], a["sums"], a["stats"], a["ws"], big, None))
+
+    for name, size in (("seq", 20), ("ref", 16)):
+        assert "dlogits overlaps" in pairs(dx=pref[name] - 508) and "margin overlaps" in pairs(margin=pref[name] + size - 4) and "seq_logp overlaps" in pairs(sums=pref[name])
+        assert "stats overlaps" in pairs(stats=pref[name] - 28) and "the workspace overlaps" in pairs(ws=pref[name])
+    assert "margin overlaps" in pairs(margin=t.logits) and "seq_logp overlaps" in pairs(sums=pref["margin"] + 4) and "stats overlaps" in pairs(stats=t.token)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [40, 9000])
+def test_outputs_next_to_inputs_are_not_overlaps(V):
+    """Per-row inputs and outputs cut out of one allocation, without a gap, give what separate ones give."""
+    from cleanmarl_amd import _native as N
+    from cleanmarl_amd import token_loss as TL
+    lib, rows = N.load(), 16
+    gen = torch.Generator().manual_seed(V)
+    x, tok = torch.randn(rows, V, generator=gen).cuda(), torch.randint(V, (rows,), generator=gen).cuda()
+    old, adv, ref, w = (torch.rand(rows, generator=gen).cuda() - 5 * (k == 0) for k in range(4))
+    want = TL.policy_loss_fwd_bwd(x, tok, old, adv, logp_ref=ref, weight=w, kl_coef=0.1)
+    need = lib.cm_token_workspace_bytes(rows, V)
+    dx, o, a, lp, r, ww, st = torch.zeros(rows * V + 5 * rows + 8, device="cuda").split([rows * V] + 5 * [rows] + [8])  # dlogits as aligned as a tensor of its own: equal bits
+    for dst, src in ((o, old), (a, adv), (r, ref), (ww, w)):
+        dst.copy_(src)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    t = N.TokenRows(x.data_ptr(), V, None, 0, tok.data_ptr(), rows, V, N.DTYPE_F32, 8, 0, 1.0)
+    N.check(lib.cm_token_policy_fwd_bwd(C.byref(t), o.data_ptr(), a.data_ptr(), r.data_ptr(), ww.data_ptr(), 0.2, 0.2, 0.1, 0.0, dx.data_ptr(), V, lp.data_ptr(), st.data_ptr(), ws.data_ptr(),
+                                        need, N.raw_stream(0)), "cm_token_policy_fwd_bwd")
+    assert torch.equal(lp, want.logp) and torch.equal(dx.view(rows, V), want.dlogits) and torch.equal(st, want.stats)
