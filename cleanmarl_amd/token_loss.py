@@ -126,7 +126,8 @@ def token_logprob_bwd(logits, token, forward, d_logp, d_entropy=None, avail=None
     ``forward``: what token_logprob(..., keep=True) returned for the same logits, token, avail and temperature.  ``out``: where the
     gradient goes; the logits themselves are allowed."""
     rows = _rows(logits, token, avail, temperature)
-    if forward.keep is None or forward.keep.shape != (*token.shape, 2) or forward.keep.device != logits.device or not forward.keep.is_contiguous():
+    kept = forward.keep
+    if kept is None or kept.dtype is not torch.float32 or kept.shape != (*token.shape, 2) or kept.device != logits.device or not kept.is_contiguous():
         raise ValueError("forward: need the result of token_logprob(..., keep=True) for these rows")
     if d_entropy is not None and forward.entropy is None:
         raise ValueError("d_entropy: the forward call has to compute the entropy (entropy=True)")
@@ -135,7 +136,7 @@ def token_logprob_bwd(logits, token, forward, d_logp, d_entropy=None, avail=None
     lib, index = N.load(), logits.get_device()
     with N.on_device(index):
         d, ld = _grad(out, logits)
-        N.check(lib.cm_token_logprob_bwd(C.byref(rows), forward.keep.data_ptr(), H, dl, dh, d.data_ptr(), ld, N.raw_stream(index)), "cm_token_logprob_bwd")
+        N.check(lib.cm_token_logprob_bwd(C.byref(rows), kept.data_ptr(), H, dl, dh, d.data_ptr(), ld, N.raw_stream(index)), "cm_token_logprob_bwd")
     return _wrote(d, out)
 
 

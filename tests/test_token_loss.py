@@ -726,3 +726,13 @@ def test_outputs_next_to_inputs_are_not_overlaps(V):
     N.check(lib.cm_token_policy_fwd_bwd(C.byref(t), o.data_ptr(), a.data_ptr(), r.data_ptr(), ww.data_ptr(), 0.2, 0.2, 0.1, 0.0, dx.data_ptr(), V, lp.data_ptr(), st.data_ptr(), ws.data_ptr(),
                                         need, N.raw_stream(0)), "cm_token_policy_fwd_bwd")
     assert torch.equal(lp, want.logp) and torch.equal(dx.view(rows, V), want.dlogits) and torch.equal(st, want.stats)
+
+
+@pytest.mark.parametrize("keep", [torch.zeros(4, 2, dtype=torch.float16), torch.zeros(4, 2, dtype=torch.float64), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(2, 4).t(), torch.zeros(4), None])
+def test_a_kept_softmax_of_another_type_is_refused(keep, monkeypatch):
+    """token_logprob_bwd reads 8 bytes of `keep` for each row: fewer (16-bit values) would be read past its end."""
+    from cleanmarl_amd import token_loss as TL
+    monkeypatch.setattr(TL, "_rows", lambda *a: None)  # (the rows themselves would have to be on a GPU)
+    row = torch.zeros(4)
+    with pytest.raises(ValueError, match="keep=True"):
+        TL.token_logprob_bwd(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64), TL.TokenLogProb(row, None, keep), row)
