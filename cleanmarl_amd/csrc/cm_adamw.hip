@@ -19,7 +19,7 @@
 namespace {
 
 constexpr int AW_BLOCK = 256, AW_TABLE = 88, AW_NT = 256, AW_CHUNK = 16;  // elements of a block; tensors of one launch; threads; blocks of one workgroup
-constexpr int AW_NORM_GRID = 1024;
+constexpr int AW_NORM_GRID = 1024, AW_MOST = (1 << 24) - 1;  // the most workgroups of a launch: it ends at 2^32 threads
 
 struct AwEntry { void* p; const void* g; void* copy; int64_t n; int first; int block; };  // first: the tensor's first workgroup; block: its first state block
 struct AwTable { AwEntry e[AW_TABLE]; uint8_t kinds[AW_TABLE]; int count; };               // kinds: dtype of param | grad << 2 | copy << 4
@@ -279,6 +279,7 @@ extern "C" int cm_adamw_multi_step(const cm_adamw_tensor_t* tensors, int n_tenso
     for (int i = 0; i < n_tensors; ++i) {
         const cm_adamw_tensor_t& t = tensors[i];
         CM_REQUIRE(t.n >= 0, "cm_adamw_multi_step: tensor %d has n=%ld", i, (long)t.n);
+        CM_REQUIRE(t.n <= (int64_t)AW_MOST * AW_CHUNK * AW_BLOCK, "cm_adamw_multi_step: %ld elements of one tensor (%d) are more than a launch takes", (long)t.n, i);
         CM_REQUIRE(aw_dtype(t.param_dtype) && aw_dtype(t.grad_dtype) && (!t.copy || aw_dtype(t.copy_dtype)), "cm_adamw_multi_step: tensor %d has an unknown dtype", i);
         CM_REQUIRE(t.n == 0 || (t.param && t.grad), "cm_adamw_multi_step: tensor %d has a NULL pointer", i);
         CM_REQUIRE(reinterpret_cast<uintptr_t>(t.param) % aw_elem(t.param_dtype) == 0 && reinterpret_cast<uintptr_t>(t.grad) % aw_elem(t.grad_dtype) == 0 &&
@@ -310,6 +311,7 @@ extern "C" int cm_adamw_multi_step(const cm_adamw_tensor_t* tensors, int n_tenso
                 const cm_adamw_tensor_t& x = tensors[i];
                 if (x.n == 0) continue;
                 const int64_t c = (cm_adamw_state_blocks(x.n) + AW_CHUNK - 1) / AW_CHUNK;
+                if (round == 1 && chunks + c > AW_MOST) break;  // the next launch's first (a tensor alone always fits); norms have a grid of their own, and room for it per AW_TABLE tensors
                 t.e[t.count] = {x.param, x.grad, x.copy, x.n, (int)chunks, (int)x.block};
                 t.kinds[t.count++] = (uint8_t)(x.param_dtype | x.grad_dtype << 2 | x.copy_dtype << 4);
                 chunks += c;  // < 2^31: the blocks of all tensors together are

@@ -212,7 +212,7 @@ extern "C" int cm_preference_fwd_bwd(const cm_token_rows_t* t, const int32_t* se
                                      float* seq_logp, float* stats, void* ws, size_t ws_bytes, cm_stream_t stream) {
     if (int rc = tok_check("cm_preference_fwd_bwd", t)) return rc;
     if (int rc = tok_check_grad("cm_preference_fwd_bwd", t, dlogits, dlogits_ld)) return rc;
-    CM_REQUIRE(pairs >= 1 && pairs <= (1 << 24), "cm_preference_fwd_bwd: pairs=%d", pairs);
+    CM_REQUIRE(pairs >= 1 && pairs < (1 << 24), "cm_preference_fwd_bwd: pairs=%d (a launch has fewer than 2^24 workgroups of 256 threads)", pairs);
     CM_REQUIRE(t->rows < ((int64_t)1 << 31), "cm_preference_fwd_bwd: rows=%ld does not fit the int32 sequence starts", (long)t->rows);
     CM_REQUIRE(seq_start && logp_ref && stats, "cm_preference_fwd_bwd: NULL seq_start / logp_ref / stats");
     CM_REQUIRE(kind == CM_PREFERENCE_SIGMOID || kind == CM_PREFERENCE_SQUARED, "cm_preference_fwd_bwd: unknown kind %d", kind);

@@ -498,3 +498,11 @@ def test_steps_from_the_parameters_own_gradients():
     assert opt.steps == 1 and bool((p < 1).all()) and bool((q == 1).all())
     opt.step([None, None])  # said so by the caller
     assert opt.steps == 2
+
+
+def test_a_tensor_of_more_workgroups_than_a_launch_has_is_refused():
+    """A launch ends at 2^32 threads, 2^24 workgroups of 256, each of 4096 elements: 2^36 elements are one too many workgroup."""
+    last = (1 << 36) - 4096  # 2^24 - 1 workgroups
+    for n in (1 << 36, last + 1):
+        assert "elements of one tensor" in _call([dict(n=n)], n_blocks=1 << 30)
+    assert "aligned" in _call([dict(n=last, grad=0x2001)], n_blocks=1 << 30)  # refused for something else

@@ -736,3 +736,14 @@ def test_a_kept_softmax_of_another_type_is_refused(keep, monkeypatch):
     row = torch.zeros(4)
     with pytest.raises(ValueError, match="keep=True"):
         TL.token_logprob_bwd(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64), TL.TokenLogProb(row, None, keep), row)
+
+
+def test_more_pairs_than_one_launch_has_workgroups_are_refused():
+    """A launch ends at 2^32 threads, 2^24 workgroups of 256; a workgroup takes one pair."""
+    from cleanmarl_amd import _native as N
+    lib, t = N.load(), _rows()
+    for pairs in (1 << 24, (1 << 31) - 1, 0, -1):
+        assert lib.cm_preference_fwd_bwd(C.byref(t), 0x20000, pairs, 0x8000000, 0.1, 0.0, 0, 1.0, 0x30000, 8, None, None, 0x40000, 0x50000, 0, None) == -1
+        assert "pairs=" in lib.cm_last_error().decode(), pairs
+    assert lib.cm_preference_fwd_bwd(C.byref(t), 0x20000, (1 << 24) - 1, 0x8000000, 0.1, 0.0, 0, 1.0, 0x30000, 8, None, None, 0x40000, 0x50000, 0, None) == -1
+    assert "workspace" in lib.cm_last_error().decode()
