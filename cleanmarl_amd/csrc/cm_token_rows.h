@@ -38,9 +38,11 @@ __device__ __forceinline__ void tok_policy_row(const TokArgs& a, const TokPolicy
     float loss = -pg - a.ent_coef * H, kl = 0.0f;
     if (a.logp_ref) {
         const float d = q.ref - logp, e = expm1f(d);
-        kl = e - d;
-        g -= a.kl_coef * e;
-        loss += a.kl_coef * kl;
+        kl = d < INFINITY ? e - d : d;  // a token that has become impossible: infinitely far, and no inf - inf
+        if (a.kl_coef != 0.0f) {        // without it the divergence is only measured: 0 * inf would reach loss and gradient
+            g -= a.kl_coef * e;
+            loss += a.kl_coef * kl;
+        }
     }
     g *= w;
     h = w * a.ent_coef;

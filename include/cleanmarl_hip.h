@@ -545,7 +545,7 @@ int cm_token_logprob_bwd(const cm_token_rows_t* t, const float* keep, const floa
                          void* dlogits, int64_t dlogits_ld, cm_stream_t stream);
 /* Clipped policy loss with a KL term, forward and backward (mappo_multienvs.py:536-570 on tokens):
  *   rho = exp(logp - logp_old), pg = min(adv rho, adv clip(rho, 1 - clip_low, 1 + clip_high)),
- *   kl = e^d - d - 1 with d = logp_ref - logp (0 without logp_ref),  loss = sum_r weight_r (-pg - entropy_coef H + kl_coef kl)
+ *   kl = e^d - d - 1 with d = logp_ref - logp (0 without logp_ref; only measured where kl_coef is 0),  loss = sum_r weight_r (-pg - entropy_coef H + kl_coef kl)
  * weight (NULL: ones) carries mask and normalisation (1 / number of tokens, or per sequence).  dlogits = dloss/dlogits.
  * stats[CM_NUM_STATS]: the weighted sums of slots CM_STAT_PG .. CM_STAT_CLIP as above, CM_STAT_LOSS, CM_STAT_COUNT = rows that count,
  * CM_STAT_KL_REF = sum weight kl, CM_STAT_WEIGHT = sum weight.  logp (may be NULL) receives the log-probabilities. */

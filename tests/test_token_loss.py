@@ -747,3 +747,25 @@ def test_more_pairs_than_one_launch_has_workgroups_are_refused():
         assert "pairs=" in lib.cm_last_error().decode(), pairs
     assert lib.cm_preference_fwd_bwd(C.byref(t), 0x20000, (1 << 24) - 1, 0x8000000, 0.1, 0.0, 0, 1.0, 0x30000, 8, None, None, 0x40000, 0x50000, 0, None) == -1
     assert "workspace" in lib.cm_last_error().decode()
+
+
+# ---------------------------------------------------------------------------------------------------------------- terms that are switched off
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [5, 700, 9000, 140003])
+def test_a_reference_without_a_coefficient_only_measures(V):
+    """kl_coef = 0 with logp_ref: the divergence is in the statistics and nowhere else, also where it is infinite (a row whose token is not available)."""
+    from cleanmarl_amd import _native as N
+    from cleanmarl_amd import token_loss as TL
+    for dtype in (torch.float32, torch.bfloat16):
+        x, tok, mask, gen = problem(6, V, dtype, V, avail=True)
+        mask[0, tok[0]] = 0
+        adv = torch.randn(6, generator=gen).cuda()
+        old, ref = torch.full((6,), -2.0).cuda(), torch.full((6,), -2.5).cuda()
+        for ent in (0.0, 0.01):
+            a = TL.policy_loss_fwd_bwd(x, tok, old, adv, avail=mask, entropy_coef=ent)
+            b = TL.policy_loss_fwd_bwd(x, tok, old, adv, logp_ref=ref, avail=mask, entropy_coef=ent)
+            assert a.logp[0].item() == -math.inf and bool(torch.isfinite(a.dlogits).all())
+            assert torch.equal(a.dlogits, b.dlogits) and torch.equal(a.logp, b.logp)
+            keep = [i for i in range(8) if i != N.STAT_KL_REF]
+            assert torch.equal(a.stats[keep].nan_to_num(7e37), b.stats[keep].nan_to_num(7e37)) and math.isfinite(b.stats[N.STAT_LOSS].item())
+            assert a.stats[N.STAT_KL_REF].item() == 0.0 and b.stats[N.STAT_KL_REF].item() == math.inf
