@@ -91,7 +91,7 @@ class Args:
     synthetic_avail_p: float = 0.7
     """ [build] availability probability of the other actions of --env_type=synthetic_shape"""
     vector_env: str = "pinned"
-    """ [build] host-env vectorisation: pinned (shared-memory workers whose blocks are page-locked and copied straight into the device rollout buffer), shm (the same workers, host-side collation) or pipe (the reference's one process + Pipe per env)"""
+    """ [build] host-env vectorisation: pinned (shared-memory workers whose blocks go through page-locked twins straight into the device rollout buffer), shm (the same workers, host-side collation) or pipe (the reference's one process + Pipe per env)"""
     env_workers: int = 0
     """ [build] worker processes of the shm vector env (0 = one per host core, at most one per env)"""
     checkpoint: str = ""

@@ -113,9 +113,9 @@ __device__ __forceinline__ float aw_block_max(float v) {
 }
 
 // Half a wave per block of 256 elements, eight to a lane: 16-byte accesses of 16-bit tensors, one 8-byte access of a block's codes.  537 M bf16
-// parameters with 8-bit states: 1.14 ms, 4.7 TB/s (a wave per block, four elements to a lane: 1.45 ms); 268 M fp32 masters, bf16 gradients and copies, 32-bit states and
-// clipping: 1.64 ms, 4.9 TB/s of the bytes that both sweeps read and write.  What is left to a large copy's 5.0 TB/s is the correctly rounded
-// square root and division, some 25 instructions each for an element.
+// parameters with 8-bit states: 1.14 ms a pass among others, 4.7 TB/s (1.17 to 1.24 behind an idle GPU; a wave per block, four elements to a lane:
+// 1.45 ms); 268 M fp32 masters, bf16 gradients and copies, 32-bit states and clipping: 1.65 ms, 4.9 TB/s of the bytes that both sweeps read and write.
+// What is left to a large copy's 5.0 TB/s is the correctly rounded square root and division, some 25 instructions each for an element.
 template <int BITS>
 __global__ __launch_bounds__(AW_NT) void k_adamw(const AwTable t, const AwArgs a) {
 #pragma clang fp contract(off)
@@ -311,7 +311,8 @@ extern "C" int cm_adamw_multi_step(const cm_adamw_tensor_t* tensors, int n_tenso
                 const cm_adamw_tensor_t& x = tensors[i];
                 if (x.n == 0) continue;
                 const int64_t c = (cm_adamw_state_blocks(x.n) + AW_CHUNK - 1) / AW_CHUNK;
-                if (round == 1 && chunks + c > AW_MOST) break;  // the next launch's first (a tensor alone always fits); norms have a grid of their own, and room for it per AW_TABLE tensors
+                // the next launch's first: a tensor alone always fits (norms have a grid of their own, and room for its sums per AW_TABLE tensors)
+                if (round == 1 && chunks + c > AW_MOST) break;
                 t.e[t.count] = {x.param, x.grad, x.copy, x.n, (int)chunks, (int)x.block};
                 t.kinds[t.count++] = (uint8_t)(x.param_dtype | x.grad_dtype << 2 | x.copy_dtype << 4);
                 chunks += c;  // < 2^31: the blocks of all tensors together are

@@ -176,8 +176,7 @@ __global__ __launch_bounds__(NT) void k_tok_sum(const TokArgs a) {
         for (int i = 0; i < TOK_STATS; ++i) { if (gridDim.x == 1) a.stats[i] = (float)st[i]; else a.part[(int64_t)blockIdx.x * TOK_STATS + i] = st[i]; }
 }
 
-// Few long rows: a row is cut into segments, a workgroup sums one, k_tok_join puts them together.  (16 rows of 131072 bf16 columns: 13.3 us with
-// a workgroup per row.)
+// Few long rows: a row is cut into segments, a workgroup sums one, k_tok_join puts them together (figures: tok_launch4, where it is chosen).
 template <class T, bool AV, bool EN, int NT>
 __global__ __launch_bounds__(NT) void k_tok_part(const TokArgs a) {
     typedef typename T::elem elem;
@@ -256,7 +255,7 @@ __global__ __launch_bounds__(NT) void k_tok_join(const TokArgs a) {
 
 // Backward only, rows too long for a wave: nothing is summed, so a workgroup takes NT * U pieces of one row, whichever.  The rows come in
 // descending order: the last ones that a forward sweep has read are the ones still in a cache.  Stores are streaming ones, they would push the logits
-// out of it (2048 x 32000 fp32, both sweeps: 160 us, so 129).  8192 x 131072 bf16 alone: 0.74 ms, 5.8 TB/s.
+// out of it (2048 x 32000 fp32, both sweeps: 160 us with ordinary ones, 129 with these).  8192 x 131072 bf16, a pass among others: 0.74 ms, 5.8 TB/s.
 template <class T, bool AV, bool EN, int NT, int U>
 __global__ __launch_bounds__(NT) void k_tok_back(const TokArgs a, int parts, int64_t tiles) {
     typedef typename T::elem elem;
@@ -655,7 +654,7 @@ int tok_launch4(TokArgs& a, void* scratch, hipStream_t s) {
         return 0;
     }
     if constexpr (MODE == TOK_LOGP) {
-        // Few long rows in segments of at least 512 pieces (8 KB).  GPU time, bf16: 16 rows of 131072 columns 14.2 -> 7.7 us, 64 rows 14.8 -> 11.1; but
+        // Few long rows in segments of at least 512 pieces (8 KB).  GPU time among other launches, bf16: 16 rows of 131072 columns 14.2 -> 7.7 us, 64 rows 14.8 -> 11.1; but
         // 128 rows of 65536 9.3 -> 11.0, 64 rows of 16384 4.5 -> 7.5: below 8192 pieces a row is done before a second launch has begun.
         if (a.rows <= TOK_SPLIT_ROWS && nfull >= 8192) {
             const int64_t most = 1024 / a.rows < nfull / 512 ? 1024 / a.rows : nfull / 512;

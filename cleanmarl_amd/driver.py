@@ -256,7 +256,7 @@ def run(script, argv=None):
         venv = PipeVectorEnv(E, dict(fac, synthetic=synth), index_offset=env_offset)
     else:
         venv = ShmVectorEnv(E, dict(fac, synthetic=synth), n_workers=args.env_workers or None, index_offset=env_offset)
-        if args.vector_env == "pinned":  # default: the workers' shared blocks are page-locked and copied straight into the device buffer
+        if args.vector_env == "pinned":  # default: the workers' shared blocks go through page-locked twins straight into the device buffer
             from .host_rollout import PinnedHostRollout
             pinned = PinnedHostRollout(venv, learner, recurrent, device, row_offset=env_offset * A)
     host_actor = HostActor(learner, A, recurrent, device, row_offset=env_offset * A)
