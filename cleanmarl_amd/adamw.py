@@ -115,7 +115,7 @@ class MultiAdamW:
             params, grads, copies = ([t[i] for i in have] for t in (params, grads, self.copies))
         else:
             copies = self.copies
-        fixed = self._fixed[have] if some else self._fixed
+        table = self._fixed[have] if some else self._fixed.view(np.uint8).copy().view(_ENTRY)  # (bytes: records are copied one by one, 12 us for 228)
         shapes, kinds = ([t[i] for i in have] for t in (self._shapes, self._dtypes)) if some else (self._shapes, self._dtypes)
         # the whole list at once (there may be hundreds of tensors); only a list that is not as it should be is looked through
         # (228 small tensors: 0.16 ms on the host with a generator for each check, 0.14 with these)
@@ -126,19 +126,16 @@ class MultiAdamW:
                 if p.shape != shape or p.dtype != kind or p.device != self.device or not p.is_contiguous():
                     raise ValueError(f"params[{i}] has another device, type, shape or layout than at the start")
                 _tensor(g, f"grads[{i}]", like=p)
-        table = np.zeros(len(have), _ENTRY)
-        for name in ("n", "block", "param_dtype", "copy_dtype"):
-            table[name] = fixed[name]
-        table["param"] = list(map(_address, params))
-        table["grad"] = list(map(_address, grads))
-        table["grad_dtype"] = list(map(_DTYPES.__getitem__, types))
+        table["param"] = np.fromiter(map(_address, params), np.uint64, len(have))
+        table["grad"] = np.fromiter(map(_address, grads), np.uint64, len(have))
+        table["grad_dtype"] = np.fromiter(map(_DTYPES.__getitem__, types), np.int32, len(have))
         if self._has_copies:
             at = [i for i, c in enumerate(copies) if c is not None]
             there = [copies[i] for i in at]
             if not (list(map(_shape, there)) == [shapes[i] for i in at] and list(map(_DTYPES.get, map(_type, there))) == table["copy_dtype"][at].tolist()
                     and all(map(_contiguous, there)) and {index}.issuperset(map(_index, there))):
                 raise ValueError("copies: one has another device, type, shape or layout than at the start")
-            table["copy"][at] = list(map(_address, there))
+            table["copy"][at] = np.fromiter(map(_address, there), np.uint64, len(at))
         lib = N.load()
         with N.on_device(index):
             clip = self.max_norm is not None and self.max_norm > 0
